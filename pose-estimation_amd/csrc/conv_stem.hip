@@ -255,7 +255,7 @@ __global__ __launch_bounds__(512, 1) void conv_stem512_kernel(const PhConvParams
           for (int nb = 0; nb < 4; nb++) a0[nb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf[nb][ks], xf[ks], a0[nb], 0, 0, 0);
 #pragma unroll
         for (int nb = 0; nb < 4; nb++) {
-          // bias as 2-vectors (packed adds), rounding two values per instruction, and the outside-the-image zero
+          // bias as 2-vectors, rounding two values per instruction, and the outside-the-image zero
           // applied to the packed words (bf16 +0 is the zero word): 10 vector operations per 4 values where the
           // element-wise form compiled to 18 -- conv1_1 is issue-bound on its SIMD (the two waves that share one
           // take turns: the second reaches barrier A 3.6 thousand cycles after the first)

@@ -53,7 +53,8 @@ __device__ __forceinline__ float lane_right(float v) {
 // (key_cnt = -1) and leaves it to the !FAST instantiation, launched right after on the same stream, whose blocks
 // return at once unless their stripe carries that mark.  (One kernel with both bodies: 88 instead of 60 registers
 // at G = 2 and 0.34 instead of 0.29 ms per 32 frames with the refine kernel; as two kernels, the fast one held to 64
-// registers: 0.27 ms.  The row body is now 29 VALU instructions for two pixels, 9 of them packed; SQ_INSTS_VALU said
+// registers: 0.27 ms.  The row body was then 29 VALU instructions for two pixels, 9 of them packed (the library is
+// built without packed fp32 instructions since: 0.226 -> 0.204 ms with the refine kernel); SQ_INSTS_VALU said
 // the kernel issued 60 per row body -- the rest was load_taps (the source rows of the next `scale` output rows and
 // the cubic's a, b, c per column group, behind chains of uniform branches) and the copies at the loop's joins; with
 // the window of source rows moved on by one in the usual case instead of searched: 50, 0.25 ms; with the bands cut
@@ -174,7 +175,7 @@ __global__ __launch_bounds__(1024) __attribute__((amdgpu_waves_per_eu(G == 4 ? 4
     return __builtin_amdgcn_readfirstlane(s_seg[i]);
   };
   auto u_val = [&](int g, float d) { return ((((ca[g] * d) * d) * d + (cb[g] * d) * d) - cc[g] * d) + tv[g][1]; };
-  // the same operations for two column groups at once, as 2-vectors (packed fp32 multiplies and adds)
+  // the same operations for two column groups at once, as 2-vectors
   typedef float nms_f2 __attribute__((ext_vector_type(2)));
   auto u_val2 = [&](int g, float d, float& u0, float& u1) {
     const nms_f2 a = {ca[g], ca[g + 1]}, bq = {cb[g], cb[g + 1]}, c = {cc[g], cc[g + 1]}, v1 = {tv[g][1], tv[g + 1][1]};
@@ -380,7 +381,7 @@ __device__ __forceinline__ float4 cubic_coef(const float* __restrict__ row, int 
 }
 // The two PAF planes of a limb are sampled at the same point, so their tables are kept INTERLEAVED -- 32 B per source
 // pixel: {a_x, a_y, b_x, b_y}, {c_x, c_y, v1_x, v1_y} -- and both planes go through cubic()'s operations as 2-vectors
-// (packed fp32 multiplies and adds: each element sees the same IEEE operations in the same order as cubic_row() / cubic() on one plane).
+// (each element sees the same IEEE operations in the same order as cubic_row() / cubic() on one plane).
 typedef float paf_f2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ paf_f2 cubic_row_cf2(const float4* row, int i1, paf_f2 d) {
   const float4 q0 = row[2 * i1], q1 = row[2 * i1 + 1];
@@ -1441,7 +1442,7 @@ int ph_launch_decode_v2(const float* net_out, int C, int hs, int ws, int Ht, int
     const int v = e ? atoi(e) : 0;
     return v == 1 || v == 2 || v == 4 ? v : 0;
   }();
-  // two columns per lane from 8 groups on: the two independent cubics pair up into packed fp32 operations
+  // two columns per lane from 8 groups on: the two independent cubics share a lane's row walk
   // (0.29 vs 0.33 ms per 32 frames at 656 columns; four per lane is no faster).  POSEHIP_NMS_G overrides.
   const int nms_g = nms_g_env ? nms_g_env : (n_groups <= 7 ? 1 : (n_groups <= 32 ? 2 : 4));
   const int nms_waves = (n_groups + nms_g - 1) / nms_g;
