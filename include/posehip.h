@@ -275,6 +275,64 @@ int ph_decode_v1_times(ph_ctx* ctx, float* ms3);
  * walk tripped). */
 int ph_decode_v1_walks(ph_ctx* ctx, int32_t* wave, int32_t* group);
 
+/* ---- 8-bit products (W8A8): no counterpart in the reference's code; what cv2.dnn's 8-bit networks compute in a layer
+ *      of kernel 1x1, with a scale for each token (row of the input: a pixel) and each output channel ----------------
+ *
+ *   s[m]   = max(f32(max_k |x[m,k]| / 127), 2^-126)          q[m,k] = round_half_even(x[m,k] / s[m]) (exact quotient)
+ *   y[m,n] = act((f32(sum_k q[m,k] w[n,k]) * ws[n]) * s[m] + bias[n])
+ *
+ * The sum is an exact int32, every operation after it is rounded to f32, the result once to its type.  A row with a NaN
+ * or an infinity gets s = NaN and q = 0: its outputs are NaN, the other rows' are not touched.
+ *
+ * These entry points take no ctx: every pointer (but the descriptors) is device memory of `device`, work is put on
+ * `stream` (NULL: the device's default stream) and nothing is waited for, allocated or kept; the calling thread's
+ * current device is left as it was.  Calls are independent of each other, also from several threads, as long as their
+ * workspaces are; all can be captured into a graph.  Workspaces: ph_w8_workspace() bytes, 256-byte aligned, free again
+ * when the call's work is done (-3: too small).  No rows (a count of 0): nothing is done. */
+#define PH_F32 0
+#define PH_F16 1
+#define PH_BF16 2
+/* Rows in three nested dimensions (of size 1 where there are fewer), strides in elements, any stride (0 too) for inputs;
+ * the values of a row are consecutive.  At most 2^31 - 1 rows. */
+typedef struct {
+  int64_t n[3];
+  int64_t stride[3];
+} ph_rows;
+/* A layer: n output channels, k inputs (k <= 131071: the int32 sum cannot overflow; n <= 2^20).  scale / bias / slope
+ * hold n values rounded up to a multiple of 16; bias may be NULL, slope may be NULL unless act is PH_ACT_PRELU. */
+typedef struct {
+  const int8_t* packed; /* ph_w8_pack's output */
+  const float* scale;
+  const float* bias;
+  const float* slope;
+  int n, k, act; /* PH_ACT_* */
+} ph_w8_layer;
+/* bytes of a packed weight (-1: sizes out of range), and the packing of int8 [n][k] (k consecutive, rows row_stride
+ * bytes apart) into the order in which the matrix instructions take it; once per weight */
+int64_t ph_w8_packed_bytes(int n, int k);
+int ph_w8_pack(int device, void* stream, const int8_t* w, int64_t row_stride, int n, int k, int8_t* packed);
+/* x: f32 / f16 / bf16 rows -> q int8 [rows][q_pitch] (16-byte aligned, q_pitch a multiple of 16 and >= k; bytes from k
+ * on are not meant for reading), scale f32 [rows] */
+int ph_w8_quantize_rows(int device, void* stream, const void* x, int x_type, const ph_rows* rows, int k, int8_t* q,
+                        int64_t q_pitch, float* scale);
+#define PH_W8_MATMUL 0
+#define PH_W8_LINEAR 1
+#define PH_W8_FEED_FORWARD 2
+/* workspace bytes of a call with m rows; h: width between the two layers of a feed-forward (else 0).  PH_W8_MATMUL needs
+ * none where q and its strides are multiples of 16 bytes. */
+int64_t ph_w8_workspace(int op, int64_t m, int k, int h, int n);
+/* 8-bit rows x layer.  out: f32 / f16 / bf16 rows of n consecutive values, out_stride[3] the strides of the same three
+ * dimensions (rows must not overlap, nor any input).  Rows of q are read in whole 16-byte pieces where they are aligned. */
+int ph_w8_matmul(int device, void* stream, const int8_t* q, const ph_rows* rows, const float* scale, const ph_w8_layer* layer,
+                 void* out, int out_type, const int64_t* out_stride, void* ws, int64_t ws_bytes);
+/* float rows x layer: ph_w8_quantize_rows + ph_w8_matmul, bit for bit */
+int ph_w8_linear(int device, void* stream, const void* x, int x_type, const ph_rows* rows, const ph_w8_layer* layer, void* out,
+                 int out_type, const int64_t* out_stride, void* ws, int64_t ws_bytes);
+/* two layers: ph_w8_linear to f32, then ph_w8_linear of that, bit for bit; layer2->k == layer1->n */
+int ph_w8_feed_forward(int device, void* stream, const void* x, int x_type, const ph_rows* rows, const ph_w8_layer* layer1,
+                       const ph_w8_layer* layer2, void* out, int out_type, const int64_t* out_stride, void* ws,
+                       int64_t ws_bytes);
+
 #ifdef __cplusplus
 }
 #endif

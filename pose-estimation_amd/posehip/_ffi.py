@@ -15,6 +15,8 @@ PH_OP_CONV, PH_OP_POOL = 0, 1
 PH_ACT_NONE, PH_ACT_RELU, PH_ACT_PRELU = 0, 1, 2
 PH_PRE_CV2, PH_PRE_NATIVE = 0, 1
 PH_NOALLOC_MAX_FRAMES = 8
+PH_F32, PH_F16, PH_BF16 = 0, 1, 2
+PH_W8_MATMUL, PH_W8_LINEAR, PH_W8_FEED_FORWARD = 0, 1, 2
 
 
 class PhBufDesc(C.Structure):
@@ -49,6 +51,15 @@ class PhV2Model(C.Structure):
 class PhV1Model(C.Structure):
     _fields_ = [("n_parts", C.c_int), ("n_limbs", C.c_int), ("pair_parts", C.c_int * 64),
                 ("mapidx", C.c_int * 64)]
+
+
+class PhRows(C.Structure):
+    _fields_ = [("n", C.c_int64 * 3), ("stride", C.c_int64 * 3)]
+
+
+class PhW8Layer(C.Structure):
+    _fields_ = [("packed", C.c_void_p), ("scale", C.c_void_p), ("bias", C.c_void_p), ("slope", C.c_void_p),
+                ("n", C.c_int), ("k", C.c_int), ("act", C.c_int)]
 
 
 # every symbol include/posehip.h declares: name -> (restype, argtypes)
@@ -105,6 +116,16 @@ SYMBOLS = {
     "ph_decode_v1_times": (C.c_int, [_vp, _fp]),
     "ph_decode_v1_walks": (C.c_int, [_vp, C.POINTER(C.c_int32), C.POINTER(C.c_int32)]),
     "ph_decode_v2_times": (C.c_int, [_vp, _fp]),
+    "ph_w8_packed_bytes": (C.c_int64, [C.c_int, C.c_int]),
+    "ph_w8_pack": (C.c_int, [C.c_int, _vp, _vp, C.c_int64, C.c_int, C.c_int, _vp]),
+    "ph_w8_quantize_rows": (C.c_int, [C.c_int, _vp, _vp, C.c_int, C.POINTER(PhRows), C.c_int, _vp, C.c_int64, _vp]),
+    "ph_w8_workspace": (C.c_int64, [C.c_int, C.c_int64, C.c_int, C.c_int, C.c_int]),
+    "ph_w8_matmul": (C.c_int, [C.c_int, _vp, _vp, C.POINTER(PhRows), _vp, C.POINTER(PhW8Layer), _vp, C.c_int,
+                               C.POINTER(C.c_int64), _vp, C.c_int64]),
+    "ph_w8_linear": (C.c_int, [C.c_int, _vp, _vp, C.c_int, C.POINTER(PhRows), C.POINTER(PhW8Layer), _vp, C.c_int,
+                               C.POINTER(C.c_int64), _vp, C.c_int64]),
+    "ph_w8_feed_forward": (C.c_int, [C.c_int, _vp, _vp, C.c_int, C.POINTER(PhRows), C.POINTER(PhW8Layer),
+                                     C.POINTER(PhW8Layer), _vp, C.c_int, C.POINTER(C.c_int64), _vp, C.c_int64]),
 }
 
 _lib = None
