@@ -318,8 +318,9 @@ int ph_w8_quantize_rows(int device, void* stream, const void* x, int x_type, con
 #define PH_W8_MATMUL 0
 #define PH_W8_LINEAR 1
 #define PH_W8_FEED_FORWARD 2
-/* workspace bytes of a call with m rows; h: width between the two layers of a feed-forward (else 0).  PH_W8_MATMUL needs
- * none where q and its strides are multiples of 16 bytes. */
+#define PH_W8_MATMUL_ANY 3
+/* workspace bytes of a call with m rows; h: width between the two layers of a feed-forward (else 0).  PH_W8_MATMUL is
+ * for rows of q that start at multiples of 16 bytes, PH_W8_MATMUL_ANY for any; many calls need none (0). */
 int64_t ph_w8_workspace(int op, int64_t m, int k, int h, int n);
 /* 8-bit rows x layer.  out: f32 / f16 / bf16 rows of n consecutive values, out_stride[3] the strides of the same three
  * dimensions (rows must not overlap, nor any input).  Rows of q are read in whole 16-byte pieces where they are aligned. */

@@ -24,13 +24,14 @@ struct PhW8Params {
   const int8_t* q;       // 8-bit rows, K contiguous values each (rows 16-byte aligned)
   PhRowMap qr;
   const float* qs;       // scale of each row [M]
-  const int8_t* w;       // packed weight fragments [N16/16][Kp/64][1024]
+  const int8_t* w;       // packed weight fragments [N16/16][K128/64][1024]
   const float* ws;       // scale of each channel [N16]
   const float* bias;     // [N16] or NULL
   const float* slope;    // [N16] or NULL
   int act;
   unsigned M;
-  int N, K, nkb, nnb;    // nkb = Kp / 64 fragments along K, nnb = N16 / 16 along N
+  int N, K, nkb, nnb;    // nkb = K128 / 64 fragments along K (even), nnb = N16 / 16 along N
   void* out;
   PhRowMap outr;
+  int* parts;            // split along K: sums [part][M][N16]
 };

@@ -151,7 +151,7 @@ static int launch_quantize_t(const T* x, const PhRowMap& xr, unsigned M, int K, 
 
 // ---- weights ---------------------------------------------------------------------------------------------------------
 
-// int8 [N][K] -> fragments of the 16 x 64 operand of the matrix instruction, [N16/16][Kp/64][lane][16]: lane l of a
+// int8 [N][K] -> fragments of the 16 x 64 operand of the matrix instruction, [N16/16][K128/64][lane][16]: lane l of a
 // fragment holds channel l % 16, k = (l / 16) * 16 .. + 15.  Rows and columns beyond N, K are zero: whatever stands
 // behind a token's last value is multiplied by zero.
 __global__ void pack_weight_kernel(const int8_t* __restrict__ w, int64_t row_stride, int N, int K, int nkb, int nnb,
@@ -185,62 +185,557 @@ __global__ void repitch_kernel(const int8_t* __restrict__ q, PhRowMap qr, unsign
 
 // ---- epilogue ----------------------------------------------------------------------------------------------------------
 
-__device__ __forceinline__ float w8_act(float v, int act, float slope) {
-  if (act == PH_ACT_RELU) return v < 0.f ? 0.f : v;
-  if (act == PH_ACT_PRELU) return v < 0.f ? v * slope : v;
+template <int ACT>
+__device__ __forceinline__ float w8_value(int acc, float ws, float s, float bias, float slope) {
+  const float v = ((float)acc * ws) * s + bias;
+  if (ACT == PH_ACT_RELU) return v < 0.f ? 0.f : v;
+  if (ACT == PH_ACT_PRELU) return v < 0.f ? v * slope : v;
   return v;
 }
-__device__ __forceinline__ float w8_value(int acc, float ws, float s, float bias, int act, float slope) {
-  return w8_act(((float)acc * ws) * s + bias, act, slope);
+// four consecutive channels of a token, rounded to the output's type; only the first `have` of them exist
+template <typename O>
+__device__ __forceinline__ void w8_store4(O* o, const f32x4 v, int have) {
+  typedef O o4 __attribute__((ext_vector_type(4), aligned(sizeof(O))));
+  if (have >= 4) {
+    o4 w;
+#pragma unroll
+    for (int e = 0; e < 4; e++) w[e] = (O)v[e];
+    *(o4*)o = w;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 3; e++)
+      if (e < have) o[e] = (O)v[e];
+  }
+}
+struct Channels {   // of four consecutive channels
+  f32x4 ws, bias, slope;
+};
+__device__ __forceinline__ Channels w8_channels(const PhW8Params& p, int n) {   // n: a multiple of 4 below N16
+  Channels c;
+  c.ws = *(const f32x4*)(p.ws + n);
+  c.bias = p.bias ? *(const f32x4*)(p.bias + n) : f32x4{0.f, 0.f, 0.f, 0.f};
+  c.slope = p.slope ? *(const f32x4*)(p.slope + n) : f32x4{0.f, 0.f, 0.f, 0.f};
+  return c;
+}
+template <int ACT>
+__device__ __forceinline__ f32x4 w8_values(const i32x4 acc, const Channels& c, float s) {
+  f32x4 v;
+#pragma unroll
+  for (int e = 0; e < 4; e++) v[e] = w8_value<ACT>(acc[e], c.ws[e], s, c.bias[e], c.slope[e]);
+  return v;
 }
 
-// ---- product: fragments straight from memory ----------------------------------------------------------------------------
-
+// one sum of four channels -> out
 template <typename O>
-__global__ __launch_bounds__(256) void w8_product_kernel(const PhW8Params p) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int fr = lane & 15, fq = lane >> 4;
-  const int nb = blockIdx.y * 4 + wave;
-  if (nb >= p.nnb) return;
-  const unsigned m0 = blockIdx.x * 64;
-  const int8_t* xp[4];
+__device__ __forceinline__ void w8_finish4(const PhW8Params& p, const i32x4 a, unsigned m, int n, float s) {
+  const Channels c = w8_channels(p, n);
+  f32x4 v;
+  if (p.act == PH_ACT_RELU) v = w8_values<PH_ACT_RELU>(a, c, s);
+  else if (p.act == PH_ACT_PRELU) v = w8_values<PH_ACT_PRELU>(a, c, s);
+  else v = w8_values<PH_ACT_NONE>(a, c, s);
+  w8_store4<O>((O*)p.out + ph_row_off(p.outr, m) + n, v, p.N - n);
+}
+
+// A wave's TM x TN fragments -> out, tokens m0 + .., channels n0 + ...  In a fragment the 16 lanes side by side hold 16
+// tokens (rows of out) and 4 channels each: stored like that, every 8-byte piece is a request of its own (13 us for a
+// 256 x 256 tile of bf16).  So two fragments' tokens at a time go through the wave's own LDS piece and leave as whole
+// rows of its channels, 16 bytes a lane.
+template <int TM, int TN, typename O>
+struct WaveOut {
+  static constexpr int ROW = TN * 16 * (int)sizeof(O);
+  static constexpr int PITCH = ROW + 16;
+  static constexpr int STEP = TM < 2 ? 1 : 2;
+  static constexpr int BYTES = STEP * 16 * PITCH;
+  typedef O oe __attribute__((ext_vector_type(16 / sizeof(O)), aligned(sizeof(O))));
+  typedef O o4 __attribute__((ext_vector_type(4)));
+
+  template <int ACT>
+  static __device__ __forceinline__ void put(const PhW8Params& p, const i32x4 (&acc)[TN][TM], unsigned m0, int n0, char* buf,
+                                             int lane) {
+    const int fr = lane & 15, fq = lane >> 4;
+    Channels c[TN];
+    float s[TM];
 #pragma unroll
-  for (int i = 0; i < 4; i++) xp[i] = p.q + ph_row_off(p.qr, min(m0 + i * 16 + fr, p.M - 1));
-  const int8_t* wp = p.w + (int64_t)nb * p.nkb * 1024 + lane * 16;
-  i32x4 acc[4] = {};
-  for (int kb = 0; kb < p.nkb; kb++) {
-    const i32x4 wf = *(const i32x4*)(wp + (int64_t)kb * 1024);
-    int k = kb * 64 + fq * 16;
-    k = k < p.K ? k : 0;   // pieces behind the row's end meet zero weights: any readable ones will do
+    for (int i = 0; i < TM; i++) s[i] = p.qs[min(m0 + i * 16 + fr, p.M - 1)];
+    const int last = p.nnb * 16 - 4;
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const i32x4 xf = *(const i32x4*)(xp[i] + k);
-      acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf, xf, acc[i], 0, 0, 0);
+    for (int j = 0; j < TN; j++) c[j] = w8_channels(p, min(n0 + j * 16 + fq * 4, last));
+    constexpr int PER = 16 / (int)sizeof(O);          // values of a 16-byte unit
+    constexpr int UNITS = STEP * 16 * (ROW / 16);     // units of a pass
+#pragma unroll
+    for (int i0 = 0; i0 < TM; i0 += STEP) {
+#pragma unroll
+      for (int i = 0; i < STEP; i++)
+#pragma unroll
+        for (int j = 0; j < TN; j++) {
+          const f32x4 v = w8_values<ACT>(acc[j][i0 + i], c[j], s[i0 + i]);
+          o4 w;
+#pragma unroll
+          for (int e = 0; e < 4; e++) w[e] = (O)v[e];
+          *(o4*)(buf + (i * 16 + fr) * PITCH + (j * 16 + fq * 4) * (int)sizeof(O)) = w;
+        }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // a wave's own pass: no other wave touches this piece
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int u0 = 0; u0 < UNITS; u0 += 64) {
+        const int u = u0 + lane, t = u / (ROW / 16), col = (u - t * (ROW / 16)) * PER;
+        const unsigned m = m0 + i0 * 16 + t;
+        const int n = n0 + col;
+        if ((UNITS % 64 == 0 || u < UNITS) && m < p.M && n < p.N) {
+          const oe w = *(const oe __attribute__((aligned(16)))*)(buf + t * PITCH + col * (int)sizeof(O));
+          O* const o = (O*)p.out + ph_row_off(p.outr, m) + n;
+          if (n + PER <= p.N) *(oe*)o = w;
+          else {
+#pragma unroll
+            for (int e = 0; e < PER - 1; e++)
+              if (n + e < p.N) o[e] = w[e];
+          }
+        }
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      __builtin_amdgcn_wave_barrier();
     }
   }
-  const int n = nb * 16 + fq * 4;
+  static __device__ __forceinline__ void store(const PhW8Params& p, const i32x4 (&acc)[TN][TM], unsigned m0, int n0, char* buf,
+                                               int lane) {
+    if (p.act == PH_ACT_RELU) put<PH_ACT_RELU>(p, acc, m0, n0, buf, lane);
+    else if (p.act == PH_ACT_PRELU) put<PH_ACT_PRELU>(p, acc, m0, n0, buf, lane);
+    else put<PH_ACT_NONE>(p, acc, m0, n0, buf, lane);
+  }
+};
+
+// ---- product: tiles through LDS ------------------------------------------------------------------------------------------
+
+typedef __attribute__((address_space(3))) void lds_void;
+typedef const __attribute__((address_space(1))) void glb_void;
+
+// Blocks go round the 8 dies in turn: each die gets a run of consecutive tiles, and a run walks 8 tiles of tokens for
+// each tile of channels, so that the tiles in flight on a die share rows and weights in its L2.
+__device__ __forceinline__ void tile_of_block(unsigned bid, unsigned mt, unsigned nt, unsigned& tm, unsigned& tn) {
+  const unsigned total = mt * nt, per = total >> 3, more = total & 7, die = bid & 7;
+  const unsigned t = die * per + min(die, more) + (bid >> 3);
+  const unsigned group = 8 * nt, g = t / group, r = t - g * group;
+  const unsigned rows = min(8u, mt - g * 8);
+  tn = r / rows;
+  tm = g * 8 + (r - tn * rows);
+}
+
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+  static_assert(N >= 0 && N < 64, "vmcnt has 6 bits");
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
+}
+
+// BM tokens x BN channels per block, WM x WN waves, a step is 128 k (two fragments), NST steps' operands in LDS.
+// Fragments are read one half step ahead of their products: while the first half's run, the second half's are read;
+// then the block meets, the slot just left is filled again, and the next step's first half is read while the second
+// half's products run.
+template <int BM, int BN, int WM, int WN, int NST, bool SPLIT, typename O>
+__global__ __launch_bounds__(64 * WM * WN) void w8_tile_kernel(const PhW8Params p, unsigned mt, unsigned nt) {
+  constexpr int WAVES = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16;
+  constexpr int XP = BM / 8, WP = BN / 8;               // 1-KiB pieces of a step
+  constexpr int XL = XP / WAVES, WL = WP / WAVES;       // pieces a wave fetches
+  static_assert(XL * WAVES == XP && WL * WAVES == WP, "pieces divide among the waves");
+  constexpr int STAGE = (XP + WP) * 1024;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave % WM, wn = wave / WM;
+  const int fr = lane & 15, fq = lane >> 4;
+  unsigned tm, tn;
+  tile_of_block(blockIdx.x, mt, nt, tm, tn);
+  const unsigned m0 = tm * BM;
+  const int nb0 = tn * (BN / 16);
+
+  const int all = p.nkb >> 1, first = SPLIT ? (int)((int64_t)all * blockIdx.y / gridDim.y) : 0;
+  const int steps = SPLIT ? (int)((int64_t)all * (blockIdx.y + 1) / gridDim.y) - first : all;   // (at least one)
+  // a piece of rows: 16 rows x 64 bytes, four lanes a row; the 16-byte unit a lane fetches is swapped in rows 4..7 and
+  // 12..15 of the piece, so that reading a fragment (16 rows, one unit each) does not hit a bank twice
+  const int unit = (lane & 3) ^ (((lane >> 4) & 1) << 1);
+  const int8_t* xsrc[XL];
+  int xk[XL];
 #pragma unroll
-  for (int i = 0; i < 4; i++) {
-    const unsigned m = m0 + i * 16 + fr;
-    if (m >= p.M) continue;
-    const float s = p.qs[m];
-    O* o = (O*)p.out + ph_row_off(p.outr, m) + n;
+  for (int u = 0; u < XL; u++) {
+    const int piece = wave + u * WAVES;
+    xsrc[u] = p.q + ph_row_off(p.qr, min(m0 + (piece >> 1) * 16 + (lane >> 2), p.M - 1));
+    xk[u] = (piece & 1) * 64 + unit * 16;
+  }
+  const int8_t* wsrc[WL];
 #pragma unroll
-    for (int e = 0; e < 4; e++)
-      if (n + e < p.N)
-        o[e] = (O)w8_value(acc[i][e], p.ws[n + e], s, p.bias ? p.bias[n + e] : 0.f, p.act, p.slope ? p.slope[n + e] : 0.f);
+  for (int u = 0; u < WL; u++) {
+    const int piece = wave + u * WAVES, nb = min(nb0 + (piece >> 1), p.nnb - 1);
+    wsrc[u] = p.w + ((int64_t)nb * p.nkb + (piece & 1)) * 1024 + lane * 16;
+  }
+  auto fetch = [&](int g, int slot) {
+    char* const st = lds + slot * STAGE;
+#pragma unroll
+    for (int u = 0; u < XL; u++) {
+      int k = (first + g) * 128 + xk[u];
+      k = k < p.K ? k : 0;   // units behind the row's end meet zero weights
+      __builtin_amdgcn_global_load_lds((glb_void*)(xsrc[u] + k), (lds_void*)(st + (wave + u * WAVES) * 1024), 16, 0, 0);
+    }
+#pragma unroll
+    for (int u = 0; u < WL; u++)
+      __builtin_amdgcn_global_load_lds((glb_void*)(wsrc[u] + (int64_t)(first + g) * 2048),
+                                       (lds_void*)(st + (XP + wave + u * WAVES) * 1024), 16, 0, 0);
+  };
+  const int xrd = wm * TM * 2048 + fr * 64 + ((fq * 16) ^ ((fr & 4) << 3));
+  const int wrd = XP * 1024 + wn * TN * 2048 + lane * 16;
+  auto read = [&](i32x4 (&xf)[TM], i32x4 (&wf)[TN], int slot, int kb) {
+    const char* const st = lds + slot * STAGE + kb * 1024;
+#pragma unroll
+    for (int j = 0; j < TN; j++) wf[j] = *(const i32x4*)(st + wrd + j * 2048);
+#pragma unroll
+    for (int i = 0; i < TM; i++) xf[i] = *(const i32x4*)(st + xrd + i * 2048);
+  };
+  i32x4 acc[TN][TM];
+#pragma unroll
+  for (int j = 0; j < TN; j++)
+#pragma unroll
+    for (int i = 0; i < TM; i++) acc[j][i] = i32x4{0, 0, 0, 0};
+  auto multiply = [&](const i32x4 (&xf)[TM], const i32x4 (&wf)[TN]) {
+#pragma unroll
+    for (int i = 0; i < TM; i++)
+#pragma unroll
+      for (int j = 0; j < TN; j++) acc[j][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[j], xf[i], acc[j][i], 0, 0, 0);
+  };
+
+#pragma unroll
+  for (int g = 0; g < NST; g++)
+    if (g < steps) fetch(g, g);
+  if (NST <= steps) wait_loads<(NST - 1) * (XL + WL)>();
+  else wait_loads<0>();
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  i32x4 xa[TM], wa[TN], xb[TM], wb[TN];
+  read(xa, wa, 0, 0);
+  int slot = 0;
+  for (int g = 0; g < steps; g++) {
+    read(xb, wb, slot, 1);
+    __builtin_amdgcn_sched_barrier(0);
+    multiply(xa, wa);
+    __builtin_amdgcn_sched_barrier(0);
+    if (g + 1 < steps) {
+      if (g + NST <= steps) wait_loads<(NST - 2) * (XL + WL)>();
+      else wait_loads<0>();
+      __builtin_amdgcn_s_barrier();   // step g + 1 is in LDS, and everybody has read all of step g
+      asm volatile("" ::: "memory");
+      const int old = slot;
+      slot = slot + 1 == NST ? 0 : slot + 1;
+      read(xa, wa, slot, 0);
+      if (g + NST < steps) fetch(g + NST, old);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    multiply(xb, wb);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  if (SPLIT) {   // sums of a part of K, joined by w8_join_kernel
+    int* const part = p.parts + (int64_t)blockIdx.y * p.M * (p.nnb * 16);
+#pragma unroll
+    for (int j = 0; j < TN; j++) {
+      const int n = (nb0 + wn * TN + j) * 16 + fq * 4;
+#pragma unroll
+      for (int i = 0; i < TM; i++) {
+        const unsigned m = m0 + (wm * TM + i) * 16 + fr;
+        if (m < p.M && n < p.N) *(i32x4*)(part + (int64_t)m * (p.nnb * 16) + n) = acc[j][i];
+      }
+    }
+    return;
+  }
+  __builtin_amdgcn_s_barrier();   // everybody has read the last step: LDS is free
+  asm volatile("" ::: "memory");
+  WaveOut<TM, TN, O>::store(p, acc, m0 + wm * TM * 16, (nb0 + wn * TN) * 16, lds + wave * WaveOut<TM, TN, O>::BYTES, lane);
+}
+
+template <int BM, int BN, int WM, int WN, int NST, bool SPLIT, typename O>
+static int launch_tile(const PhW8Params& p, int parts, hipStream_t st) {
+  constexpr int ring = NST * (BM + BN) * 128, tile = WM * WN * WaveOut<BM / WM / 16, BN / WN / 16, O>::BYTES;
+  constexpr int lds = ring > tile ? ring : tile;
+  static int granted[PH_MAX_DEVICES];
+  const void* fn = (const void*)w8_tile_kernel<BM, BN, WM, WN, NST, SPLIT, O>;
+  if (lds > 64 * 1024 && ph_ensure_lds(fn, lds, granted)) return -1;
+  const unsigned mt = (p.M + BM - 1) / BM, nt = (p.N + BN - 1) / BN;
+  hipLaunchKernelGGL((w8_tile_kernel<BM, BN, WM, WN, NST, SPLIT, O>), dim3(mt * nt, SPLIT ? parts : 1), dim3(64 * WM * WN), lds, st, p, mt, nt);
+  PH_CHECK(hipGetLastError());
+  return 0;
+}
+
+// ---- product: few tokens -------------------------------------------------------------------------------------------------
+//
+// Up to 64 tokens: the weights are read once, each fragment by one wave straight into registers (a fragment is 1 KiB in
+// one piece), and the rows, which every block needs, come from cache.  A block has 16 channels; its waves take fragments
+// along K in turn and their sums meet in LDS.
+//
+// T is int8_t, or the type of float rows that the block quantises itself, into LDS, while its first weights are on their
+// way: for one to a few tokens that costs less than a launch of its own before this one (see launch_few_float).
+struct FloatRows {
+  const void* x;
+  PhRowMap r;
+  int vec;   // rows are 16-byte aligned
+};
+
+template <typename T>
+__device__ __forceinline__ void load8(const T* row, int k, int K, bool vec, float* o) {
+  if (vec && k + 8 <= K) {
+    const Vec8<T> c = *(const Vec8<T>*)(row + k);
+#pragma unroll
+    for (int i = 0; i < 8; i++) o[i] = c.get(i);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; i++) o[i] = k + i < K ? to_f32(row[k + i]) : 0.f;
+  }
+}
+
+// M <= 8 rows -> int8 rows of `pitch` bytes and their scales in LDS; W waves, W / (M rounded up to a power of two) a row
+template <int W, typename T>
+__device__ __forceinline__ void quantize_block(const FloatRows& f, unsigned M, int K, char* q, int pitch, float* scale,
+                                               unsigned* amax, int wave, int lane) {
+  const T* const x = (const T*)f.x;
+  const unsigned per = M > 4 ? 1 : M > 2 ? 2 : M > 1 ? 4 : 8;   // waves of a row (W = 8)
+  static_assert(W == 8, "waves are dealt to rows for 8");
+  const unsigned row = wave / per;
+  const bool has = row < M;
+  const T* const xr = x + ph_row_off(f.r, has ? row : 0);
+  const int k0 = ((wave % per) * 64 + lane) * 8, step = per * 512;
+  float first[8];
+  unsigned am = 0;
+  if (has) {
+    for (int k = k0; k < K; k += step) {
+      float v[8];
+      load8(xr, k, K, f.vec, v);
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        am = max(am, abs_bits(v[i]));
+        if (k == k0) first[i] = v[i];
+      }
+    }
+  }
+#pragma unroll
+  for (int d = 32; d; d >>= 1) am = max(am, (unsigned)__shfl_xor((int)am, d));
+  if (lane == 0) amax[wave] = am;
+  __syncthreads();
+  if (has) {
+    am = 0;
+    for (unsigned w = 0; w < per; w++) am = max(am, amax[row * per + w]);
+    bool finite;
+    const RowScale r = row_scale(am, finite);
+    if (lane == 0 && wave % per == 0) scale[row] = finite ? r.s : __uint_as_float(0x7fc00000u);
+    for (int k = k0; k < K; k += step) {
+      float v[8];
+      if (k == k0) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = first[i];
+      } else {
+        load8(xr, k, K, f.vec, v);
+      }
+      union { int8_t b[8]; uint64_t u; } o;
+#pragma unroll
+      for (int i = 0; i < 8; i++) o.b[i] = finite ? (int8_t)quant_one(v[i], r) : (int8_t)0;
+      *(uint64_t*)(q + (int)row * pitch + k) = o.u;
+    }
+  }
+  __syncthreads();
+}
+
+template <int TM, int W, bool SPLIT, typename T, typename O>
+__global__ __launch_bounds__(64 * W) void w8_few_kernel(const PhW8Params p, const FloatRows f) {
+  constexpr bool FLOAT = !__is_same(T, int8_t);
+  constexpr int DEPTH = 4;   // fragments of weights in flight per wave
+  __shared__ __attribute__((aligned(16))) int red[W][TM][256];
+  extern __shared__ __attribute__((aligned(16))) char s_q[];   // FLOAT: the rows in 8 bits
+  __shared__ float s_scale[8];
+  __shared__ unsigned s_amax[W];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int fr = lane & 15, fq = lane >> 4;
+  const int nb = blockIdx.x;
+  const int kb0 = SPLIT ? (int)((int64_t)p.nkb * blockIdx.y / gridDim.y) : 0;
+  const int kb1 = SPLIT ? (int)((int64_t)p.nkb * (blockIdx.y + 1) / gridDim.y) : p.nkb;
+  const int8_t* const wp = p.w + (int64_t)nb * p.nkb * 1024 + lane * 16;
+  i32x4 wf[DEPTH];
+  auto weights = [&](int kb) {
+#pragma unroll
+    for (int d = 0; d < DEPTH; d++)
+      if (kb + d * W < kb1) wf[d] = __builtin_nontemporal_load((const i32x4*)(wp + (int64_t)(kb + d * W) * 1024));
+  };
+  weights(kb0 + wave);
+  const int pitch = p.nkb * 64 + 16;   // (16 rows at one multiple of 64 bytes would share their banks)
+  if constexpr (FLOAT) quantize_block<W, T>(f, p.M, p.K, s_q, pitch, s_scale, s_amax, wave, lane);
+  const int8_t* xp[TM];   // (FLOAT: one fragment of tokens, in LDS)
+  const char* const xq = s_q + min((unsigned)fr, p.M - 1) * pitch;
+#pragma unroll
+  for (int i = 0; i < TM; i++) xp[i] = FLOAT ? nullptr : p.q + ph_row_off(p.qr, min((unsigned)(i * 16 + fr), p.M - 1));
+  i32x4 acc[TM];
+#pragma unroll
+  for (int i = 0; i < TM; i++) acc[i] = i32x4{0, 0, 0, 0};
+  for (int kb = kb0 + wave; kb < kb1; kb += W * DEPTH) {
+    i32x4 xf[DEPTH][TM], w[DEPTH];
+#pragma unroll
+    for (int d = 0; d < DEPTH; d++) {
+      int k = (kb + d * W) * 64 + fq * 16;
+      k = k < p.K ? k : 0;   // units behind the row's end meet zero weights
+#pragma unroll
+      for (int i = 0; i < TM; i++) {
+        if constexpr (FLOAT) xf[d][i] = *(const i32x4*)(xq + k);
+        else xf[d][i] = *(const i32x4*)(xp[i] + k);
+      }
+      w[d] = wf[d];
+    }
+    weights(kb + W * DEPTH);
+#pragma unroll
+    for (int d = 0; d < DEPTH; d++)
+      if (kb + d * W < kb1)
+#pragma unroll
+        for (int i = 0; i < TM; i++) acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[d], xf[d][i], acc[i], 0, 0, 0);
+  }
+#pragma unroll
+  for (int i = 0; i < TM; i++) *(i32x4*)&red[wave][i][lane * 4] = acc[i];
+  __syncthreads();
+  if (wave < TM) {
+    i32x4 a = *(const i32x4*)&red[0][wave][lane * 4];
+#pragma unroll
+    for (int w = 1; w < W; w++) a += *(const i32x4*)&red[w][wave][lane * 4];
+    const unsigned m = wave * 16 + fr;
+    const int n = nb * 16 + fq * 4;
+    if (m >= p.M || n >= p.N) return;
+    if (SPLIT) *(i32x4*)(p.parts + ((int64_t)blockIdx.y * p.M + m) * (p.nnb * 16) + n) = a;
+    else w8_finish4<O>(p, a, m, n, FLOAT ? s_scale[m & 7] : p.qs[m]);
+  }
+}
+
+// sums of the parts of K -> out; integers, so that their order does not matter
+template <typename O>
+__global__ __launch_bounds__(256) void w8_join_kernel(const PhW8Params p, int parts) {
+  const int q4 = (p.N + 3) / 4;
+  const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (t >= (int64_t)p.M * q4) return;
+  const unsigned m = (unsigned)(t / q4);
+  const int n = (int)(t - (int64_t)m * q4) * 4;
+  const int64_t pitch = (int64_t)p.M * (p.nnb * 16);
+  const int* at = p.parts + (int64_t)m * (p.nnb * 16) + n;
+  i32x4 a = i32x4{0, 0, 0, 0};
+  for (int s0 = 0; s0 < parts; s0 += 8) {   // eight at a time on their way
+    i32x4 b[8];
+#pragma unroll
+    for (int s = 0; s < 8; s++) b[s] = s0 + s < parts ? *(const i32x4*)(at + (s0 + s) * pitch) : i32x4{0, 0, 0, 0};
+#pragma unroll
+    for (int s = 0; s < 8; s++) a += b[s];
+  }
+  w8_finish4<O>(p, a, m, n, p.qs[m]);
+}
+
+template <int TM, bool SPLIT, typename O>
+static int launch_few(const PhW8Params& p, int parts, hipStream_t st) {
+  hipLaunchKernelGGL((w8_few_kernel<TM, 8, SPLIT, int8_t, O>), dim3(p.nnb, SPLIT ? parts : 1), dim3(512), 0, st, p, FloatRows{});
+  PH_CHECK(hipGetLastError());
+  return 0;
+}
+
+// What a product costs by each kernel, in us, as measured: a block's step of 128 k alone on its CU (`alone`) and with
+// the CU full (`full`), what a round of blocks costs beside its steps (`fixed`), blocks that fit a CU (`fit`).
+//   4096^3, us: 256x256 60, 128x128 69 (three slots: 84), 128x64 84, 64x64 99
+//   1024 x 4096 x 4096: 128x128 24 (three slots: 22), 128x64 23, 64x64 29;  512: 128x64 21, 64x64 16
+//   61 x 32500 x 187: 64x64 in one piece 50, in 4 parts 22, in 16 parts 11
+struct Kernel {
+  int bm, bn, fit;
+  float alone, full, fixed;
+};
+enum { K_256, K_128, K_128_3, K_128x64, K_64, K_FEW, N_KERNELS = K_FEW };
+static const Kernel kernels[N_KERNELS] = {
+    {256, 256, 1, 1.72f, 1.72f, 6.f}, {128, 128, 2, 0.64f, 0.50f, 3.5f}, {128, 128, 1, 0.56f, 0.56f, 3.5f},
+    {128, 64, 3, 0.55f, 0.32f, 2.6f}, {64, 64, 3, 0.32f, 0.20f, 2.2f}};
+
+struct Choice {
+  int kernel, parts;
+};
+// Splitting K pays where there are far fewer blocks than CUs: the parts' sums (4 bytes each) are written, read and
+// joined by a second launch.
+static Choice choose(int64_t M, int N, int nkb) {
+  const int steps = nkb / 2;
+  const int64_t n16 = (N + 15) / 16 * 16;
+  const float wire = (float)n16 * nkb * 64 / 5.5e6f;   // the weights, once, from memory
+  auto join = [&](int parts) { return parts > 1 ? 3.3f + (float)M * n16 * 4e-6f * parts / 2.f : 0.f; };   // (2 TB/s)
+  Choice best = {K_64, 1};
+  float least = 1e30f;
+  for (int parts = 1; parts <= 32 && parts <= steps; parts *= 2) {
+    if (parts > 1 && (float)M * n16 * parts > (float)(1 << 24)) break;
+    const int s = (steps + parts - 1) / parts;
+    for (int k = 0; k < N_KERNELS; k++) {
+      const Kernel& c = kernels[k];
+      const int64_t blocks = (M + c.bm - 1) / c.bm * ((N + c.bn - 1) / c.bn) * parts;
+      const int64_t each = (blocks + 255) / 256, rounds = (each + c.fit - 1) / c.fit;
+      const float run = (float)s * (each * c.full > rounds * c.alone ? each * c.full : rounds * c.alone);
+      const float t = (run > wire ? run : wire) + rounds * c.fixed + join(parts);
+      if (t < least) least = t, best = {k, parts};
+    }
+    if (M <= 64) {   // a wave's step is one fragment of 64 k; blocks' loads share the memory's rate
+      const int tm = (int)(M + 15) / 16;
+      const int64_t blocks = n16 / 16 * parts, rounds = (blocks + 511) / 512;
+      const float run = (s * 2 + 31) / 32 * rounds * (0.35f + 0.45f * tm), w = wire * (0.8f + 0.2f * tm);
+      const float t = 1.f + 0.5f * tm + (run > w ? run : w) + join(parts);
+      if (t < least) least = t, best = {K_FEW, parts};
+    }
+  }
+  return best;
+}
+
+static int64_t parts_bytes(int64_t M, int N, int nkb) {
+  const Choice c = choose(M, N, nkb);
+  return c.parts > 1 ? (int64_t)c.parts * M * ((N + 15) / 16 * 16) * 4 : 0;
+}
+
+template <bool SPLIT, typename O>
+static int launch_kernel(const PhW8Params& p, const Choice& c, hipStream_t st) {
+  switch (c.kernel) {
+    case K_256: return launch_tile<256, 256, 2, 4, 2, SPLIT, O>(p, c.parts, st);
+    case K_128: return launch_tile<128, 128, 2, 4, 2, SPLIT, O>(p, c.parts, st);
+    case K_128_3: return launch_tile<128, 128, 2, 4, 3, SPLIT, O>(p, c.parts, st);
+    case K_128x64: return launch_tile<128, 64, 4, 2, 2, SPLIT, O>(p, c.parts, st);
+    case K_64: return launch_tile<64, 64, 2, 2, 3, SPLIT, O>(p, c.parts, st);
+    default:
+      if (p.M <= 16) return launch_few<1, SPLIT, O>(p, c.parts, st);
+      if (p.M <= 32) return launch_few<2, SPLIT, O>(p, c.parts, st);
+      if (p.M <= 48) return launch_few<3, SPLIT, O>(p, c.parts, st);
+      return launch_few<4, SPLIT, O>(p, c.parts, st);
+  }
+}
+
+// parts_bytes() of workspace at p.parts
+template <typename O>
+static int launch_product_t(const PhW8Params& p, hipStream_t st) {
+  const Choice c = choose(p.M, p.N, p.nkb);
+  if (c.parts == 1) return launch_kernel<false, O>(p, c, st);
+  if (launch_kernel<true, O>(p, c, st)) return -1;
+  const int64_t pieces = (int64_t)p.M * ((p.N + 3) / 4);
+  hipLaunchKernelGGL((w8_join_kernel<O>), dim3((unsigned)((pieces + 255) / 256)), dim3(256), 0, st, p, c.parts);
+  PH_CHECK(hipGetLastError());
+  return 0;
+}
+
+// Up to 8 tokens of up to 32 K values in all: the product's blocks quantise the rows themselves.
+static bool few_float(int64_t M, int K) { return M <= 8 && M * K <= 32768; }
+
+template <typename T, typename O>
+static int launch_few_float_t(const PhW8Params& p, const FloatRows& f, hipStream_t st) {
+  const int lds = (int)p.M * (p.nkb * 64 + 16);   // at most 34 KB
+  hipLaunchKernelGGL((w8_few_kernel<1, 8, false, T, O>), dim3(p.nnb), dim3(512), lds, st, p, f);
+  PH_CHECK(hipGetLastError());
+  return 0;
+}
+template <typename O>
+static int launch_few_float(const PhW8Params& p, int x_type, const FloatRows& f, hipStream_t st) {
+  switch (x_type) {
+    case PH_F32: return launch_few_float_t<float, O>(p, f, st);
+    case PH_F16: return launch_few_float_t<_Float16, O>(p, f, st);
+    default: return launch_few_float_t<bf16, O>(p, f, st);
   }
 }
 
 static int launch_product(const PhW8Params& p, int out_type, hipStream_t st) {
-  const dim3 grid((p.M + 63) / 64, (p.nnb + 3) / 4), block(256);
   switch (out_type) {
-    case PH_F32: hipLaunchKernelGGL((w8_product_kernel<float>), grid, block, 0, st, p); break;
-    case PH_F16: hipLaunchKernelGGL((w8_product_kernel<_Float16>), grid, block, 0, st, p); break;
-    default: hipLaunchKernelGGL((w8_product_kernel<bf16>), grid, block, 0, st, p); break;
+    case PH_F32: return launch_product_t<float>(p, st);
+    case PH_F16: return launch_product_t<_Float16>(p, st);
+    default: return launch_product_t<bf16>(p, st);
   }
-  PH_CHECK(hipGetLastError());
-  return 0;
 }
 
 // ---- entry points --------------------------------------------------------------------------------------------------------
@@ -272,6 +767,7 @@ struct DeviceScope {
 
 int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 int64_t q_pitch_of(int64_t K) { return up(K, 16); }
+int nkb_of(int k) { return (int)(up(k, 128) / 64); }
 
 PhRowMap row_map(const ph_rows& r) {
   PhRowMap m;
@@ -342,10 +838,11 @@ int quantize(const void* x, int type, const PhRowMap& xr, unsigned M, int K, int
 }
 
 PhW8Params product_params(const int8_t* q, const PhRowMap& qr, const float* qs, unsigned M, const ph_w8_layer& l, void* out,
-                          const PhRowMap& outr) {
+                          const PhRowMap& outr, int* parts) {
   PhW8Params p;
   p.q = q, p.qr = qr, p.qs = qs, p.w = l.packed, p.ws = l.scale, p.bias = l.bias, p.slope = l.slope, p.act = l.act;
-  p.M = M, p.N = l.n, p.K = l.k, p.nkb = (l.k + 63) / 64, p.nnb = (l.n + 15) / 16, p.out = out, p.outr = outr;
+  p.parts = parts;
+  p.M = M, p.N = l.n, p.K = l.k, p.nkb = nkb_of(l.k), p.nnb = (l.n + 15) / 16, p.out = out, p.outr = outr;
   return p;
 }
 
@@ -375,7 +872,7 @@ int64_t ph_w8_packed_bytes(int n, int k) {
     ph_set_error("ph_w8_packed_bytes: 1 <= n <= %d and 1 <= k <= %d, got %d and %d", W8_MAX_N, W8_MAX_K, n, k);
     return -1;
   }
-  return up(n, 16) * up(k, 64);
+  return up(n, 16) * up(k, 128);
 }
 
 int ph_w8_pack(int device, void* stream, const int8_t* w, int64_t row_stride, int n, int k, int8_t* packed) {
@@ -385,7 +882,7 @@ int ph_w8_pack(int device, void* stream, const int8_t* w, int64_t row_stride, in
     return -1;
   }
   W8_DEVICE(device);
-  const int nkb = (k + 63) / 64, nnb = (n + 15) / 16;
+  const int nkb = nkb_of(k), nnb = (n + 15) / 16;
   const int64_t pieces = (int64_t)nkb * nnb * 64;
   hipLaunchKernelGGL(pack_weight_kernel, dim3((unsigned)((pieces + 255) / 256)), dim3(256), 0, (hipStream_t)stream, w,
                      row_stride, n, k, nkb, nnb, packed);
@@ -409,26 +906,40 @@ int ph_w8_quantize_rows(int device, void* stream, const void* x, int x_type, con
 }
 
 int64_t ph_w8_workspace(int op, int64_t m, int k, int h, int n) {
-  if (m < 0 || m > 0x7fffffff || k < 1 || h < 0 || n < 1) {
+  if (m < 0 || m > 0x7fffffff || k < 1 || k > W8_MAX_K || h < 0 || h > W8_MAX_K || n < 1 || n > W8_MAX_N) {
     ph_set_error("ph_w8_workspace: bad sizes");
     return -1;
   }
+  if (m == 0) return 0;
   Pieces w = {nullptr};
   switch (op) {
-    case PH_W8_MATMUL:   // rows that are not 16-byte aligned are laid out anew
+    case PH_W8_MATMUL:
+      w.take<char>(parts_bytes(m, n, nkb_of(k)));
+      break;
+    case PH_W8_MATMUL_ANY:   // rows that are not 16-byte aligned are laid out anew
+      w.take<char>(parts_bytes(m, n, nkb_of(k)));
       w.take<int8_t>(m * q_pitch_of(k));
       break;
     case PH_W8_LINEAR:
+      if (few_float(m, k)) break;
+      w.take<char>(parts_bytes(m, n, nkb_of(k)));
       w.take<int8_t>(m * q_pitch_of(k));
       w.take<float>(m);
       break;
-    case PH_W8_FEED_FORWARD:
+    case PH_W8_FEED_FORWARD: {
+      if (h < 1) {
+        ph_set_error("ph_w8_workspace: a feed-forward's inner width is 1 or more");
+        return -1;
+      }
+      const int64_t a = parts_bytes(m, h, nkb_of(k)), b = parts_bytes(m, n, nkb_of(h));
+      w.take<char>(a > b ? a : b);   // (the two products run one after the other)
       w.take<int8_t>(m * q_pitch_of(k));
       w.take<float>(m);
       w.take<float>(m * up(h, 4));
       w.take<int8_t>(m * q_pitch_of(h));
       w.take<float>(m);
       break;
+    }
     default:
       ph_set_error("ph_w8_workspace: unknown operator %d", op);
       return -1;
@@ -453,17 +964,20 @@ int ph_w8_matmul(int device, void* stream, const int8_t* q, const ph_rows* rows,
   for (int d = 0; d < 3; d++) orow.stride[d] = out_stride[d];
   PhRowMap qr = row_map(*rows);
   const bool direct = aligned16(q, qr, 1);
-  if (!direct && !ws_ok(who, ws, ws_bytes, ph_w8_workspace(PH_W8_MATMUL, M, layer->k, 0, layer->n))) return -3;
+  if (!ws_ok(who, ws, ws_bytes, ph_w8_workspace(direct ? PH_W8_MATMUL : PH_W8_MATMUL_ANY, M, layer->k, 0, layer->n))) return -3;
   W8_DEVICE(device);
+  Pieces w = {(char*)ws};
+  int* parts = (int*)w.take<char>(parts_bytes(M, layer->n, nkb_of(layer->k)));
   if (!direct) {
     const int64_t pitch = q_pitch_of(layer->k), pieces = M * (pitch / 16);
+    int8_t* even = w.take<int8_t>(M * pitch);
     hipLaunchKernelGGL(repitch_kernel, dim3((unsigned)((pieces + 255) / 256)), dim3(256), 0, (hipStream_t)stream, q, qr,
-                       (unsigned)M, layer->k, (int8_t*)ws, pitch);
+                       (unsigned)M, layer->k, even, pitch);
     PH_CHECK(hipGetLastError());
-    q = (const int8_t*)ws;
+    q = even;
     qr = even_rows(pitch);
   }
-  return launch_product(product_params(q, qr, scale, (unsigned)M, *layer, out, row_map(orow)), out_type, (hipStream_t)stream);
+  return launch_product(product_params(q, qr, scale, (unsigned)M, *layer, out, row_map(orow), parts), out_type, (hipStream_t)stream);
 }
 
 int ph_w8_linear(int device, void* stream, const void* x, int x_type, const ph_rows* rows, const ph_w8_layer* layer, void* out,
@@ -477,13 +991,24 @@ int ph_w8_linear(int device, void* stream, const void* x, int x_type, const ph_r
   ph_rows orow = *rows;
   for (int d = 0; d < 3; d++) orow.stride[d] = out_stride[d];
   W8_DEVICE(device);
+  hipStream_t st = (hipStream_t)stream;
+  const PhRowMap xr = row_map(*rows), outr = row_map(orow);
+  if (few_float(M, layer->k)) {
+    const FloatRows f = {x, xr, aligned16(x, xr, x_type == PH_F32 ? 4 : 2)};
+    const PhW8Params p = product_params(nullptr, xr, nullptr, (unsigned)M, *layer, out, outr, nullptr);
+    switch (out_type) {
+      case PH_F32: return launch_few_float<float>(p, x_type, f, st);
+      case PH_F16: return launch_few_float<_Float16>(p, x_type, f, st);
+      default: return launch_few_float<bf16>(p, x_type, f, st);
+    }
+  }
   const int64_t pitch = q_pitch_of(layer->k);
   Pieces w = {(char*)ws};
+  int* parts = (int*)w.take<char>(parts_bytes(M, layer->n, nkb_of(layer->k)));
   int8_t* q = w.take<int8_t>(M * pitch);
   float* s = w.take<float>(M);
-  if (quantize(x, x_type, row_map(*rows), (unsigned)M, layer->k, q, pitch, s, (hipStream_t)stream)) return -1;
-  return launch_product(product_params(q, even_rows(pitch), s, (unsigned)M, *layer, out, row_map(orow)), out_type,
-                        (hipStream_t)stream);
+  if (quantize(x, x_type, xr, (unsigned)M, layer->k, q, pitch, s, st)) return -1;
+  return launch_product(product_params(q, even_rows(pitch), s, (unsigned)M, *layer, out, outr, parts), out_type, st);
 }
 
 int ph_w8_feed_forward(int device, void* stream, const void* x, int x_type, const ph_rows* rows, const ph_w8_layer* layer1,
@@ -506,15 +1031,17 @@ int ph_w8_feed_forward(int device, void* stream, const void* x, int x_type, cons
   const int K = layer1->k, H = layer1->n;
   const int64_t pitch = q_pitch_of(K), hpitch = up(H, 4), pitch2 = q_pitch_of(H);
   Pieces w = {(char*)ws};
+  const int64_t pa = parts_bytes(M, H, nkb_of(K)), pb = parts_bytes(M, layer2->n, nkb_of(H));
+  int* parts = (int*)w.take<char>(pa > pb ? pa : pb);
   int8_t* q = w.take<int8_t>(M * pitch);
   float* s = w.take<float>(M);
   float* h = w.take<float>(M * hpitch);
   int8_t* q2 = w.take<int8_t>(M * pitch2);
   float* s2 = w.take<float>(M);
   if (quantize(x, x_type, row_map(*rows), (unsigned)M, K, q, pitch, s, st)) return -1;
-  if (launch_product(product_params(q, even_rows(pitch), s, (unsigned)M, *layer1, h, even_rows(hpitch)), PH_F32, st)) return -1;
+  if (launch_product(product_params(q, even_rows(pitch), s, (unsigned)M, *layer1, h, even_rows(hpitch), parts), PH_F32, st)) return -1;
   if (quantize(h, PH_F32, even_rows(hpitch), (unsigned)M, H, q2, pitch2, s2, st)) return -1;
-  return launch_product(product_params(q2, even_rows(pitch2), s2, (unsigned)M, *layer2, out, row_map(orow)), out_type, st);
+  return launch_product(product_params(q2, even_rows(pitch2), s2, (unsigned)M, *layer2, out, row_map(orow), parts), out_type, st);
 }
 
 }  // extern "C"

@@ -16,7 +16,7 @@ PH_ACT_NONE, PH_ACT_RELU, PH_ACT_PRELU = 0, 1, 2
 PH_PRE_CV2, PH_PRE_NATIVE = 0, 1
 PH_NOALLOC_MAX_FRAMES = 8
 PH_F32, PH_F16, PH_BF16 = 0, 1, 2
-PH_W8_MATMUL, PH_W8_LINEAR, PH_W8_FEED_FORWARD = 0, 1, 2
+PH_W8_MATMUL, PH_W8_LINEAR, PH_W8_FEED_FORWARD, PH_W8_MATMUL_ANY = 0, 1, 2, 3
 
 
 class PhBufDesc(C.Structure):

@@ -227,10 +227,9 @@ def matmul(q, scale, layer, out=None, dtype=None):
     y = _output(q, layer.n, out, dtype or (torch.bfloat16 if out is None else None))
     rows, ostride, m = _out_rows(q.shape, q.stride(), y.shape, y.stride())
     if m:
-        ws, need = None, 0
-        if q.data_ptr() % 16 or rows.stride[0] % 16 or rows.stride[1] % 16 or rows.stride[2] % 16:
-            need = _workspace(_ffi.PH_W8_MATMUL, m, layer.k, 0, layer.n)
-            ws = torch.empty(need, dtype=torch.int8, device=q.device)
+        even = not (q.data_ptr() % 16 or rows.stride[0] % 16 or rows.stride[1] % 16 or rows.stride[2] % 16)
+        need = _workspace(_ffi.PH_W8_MATMUL if even else _ffi.PH_W8_MATMUL_ANY, m, layer.k, 0, layer.n)
+        ws = torch.empty(need, dtype=torch.int8, device=q.device) if need else None
         _ffi.check(_ffi.lib().ph_w8_matmul(q.device.index, _stream(q.device), q.data_ptr(), rows, scale.data_ptr(), layer.desc,
                                            y.data_ptr(), _TYPES[y.dtype], ostride, ws.data_ptr() if need else None, need),
                    "ph_w8_matmul")
@@ -246,9 +245,10 @@ def linear(x, layer, out=None, dtype=None):
     rows, ostride, m = _out_rows(x.shape, x.stride(), y.shape, y.stride())
     if m:
         need = _workspace(_ffi.PH_W8_LINEAR, m, layer.k, 0, layer.n)
-        ws = torch.empty(need, dtype=torch.int8, device=x.device)
+        ws = torch.empty(need, dtype=torch.int8, device=x.device) if need else None
         _ffi.check(_ffi.lib().ph_w8_linear(x.device.index, _stream(x.device), x.data_ptr(), _TYPES[x.dtype], rows, layer.desc,
-                                           y.data_ptr(), _TYPES[y.dtype], ostride, ws.data_ptr(), need), "ph_w8_linear")
+                                           y.data_ptr(), _TYPES[y.dtype], ostride, ws.data_ptr() if need else None, need),
+                   "ph_w8_linear")
     return y
 
 
