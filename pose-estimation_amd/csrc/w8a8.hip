@@ -12,137 +12,142 @@
 
 // ---- quantisation of rows ------------------------------------------------------------------------------------------
 
-template <typename T>
-__device__ __forceinline__ float to_f32(T v) { return (float)v; }
-
 // |v| as an integer that orders like it; NaN and infinities are >= 0x7f800000
 __device__ __forceinline__ unsigned abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 
 struct RowScale {
   float s, inv, half;   // scale, 1 / scale, scale / 2
+  bool finite;
 };
-__device__ __forceinline__ RowScale row_scale(unsigned amax_bits, bool& finite) {
-  finite = amax_bits < 0x7f800000u;
+__device__ __forceinline__ RowScale row_scale(unsigned amax_bits) {
   RowScale r;
-  r.s = finite ? fmaxf(__uint_as_float(amax_bits) / 127.f, 0x1p-126f) : 1.f;
+  r.finite = amax_bits < 0x7f800000u;
+  r.s = r.finite ? fmaxf(__uint_as_float(amax_bits) / 127.f, 0x1p-126f) : 1.f;
   r.inv = 1.f / r.s;
   r.half = 0.5f * r.s;
   return r;
 }
-// round_half_even(x / s): x * (1/s) is within 127 * 2^-23 of the quotient, so its rounding is the wanted number or its
-// neighbour; the remainder x - q s is exact in one fused operation and tells which.
-__device__ __forceinline__ int quant_one(float x, const RowScale& r) {
-  const float q = rintf(x * r.inv);
-  const float rem = __builtin_fmaf(-q, r.s, x);
-  const float a = fabsf(rem);
-  const int qi = (int)q;
-  const bool move = a > r.half || (a == r.half && (qi & 1));
-  return qi + (move ? (rem > 0.f ? 1 : -1) : 0);
-}
+__device__ __forceinline__ float scale_out(const RowScale& r) { return r.finite ? r.s : __uint_as_float(0x7fc00000u); }
 
-template <typename T>
-struct Vec8;
-template <>
-struct Vec8<float> {
-  f32x4 a, b;
-  __device__ __forceinline__ float get(int i) const { return i < 4 ? a[i] : b[i - 4]; }
-};
-template <>
-struct Vec8<_Float16> {
-  _Float16 v __attribute__((ext_vector_type(8)));
-  __device__ __forceinline__ float get(int i) const { return (float)v[i]; }
-};
-template <>
-struct Vec8<bf16> {
-  bf16x8 v;
-  __device__ __forceinline__ float get(int i) const { return (float)v[i]; }
-};
-
-// A group of 64 * NW threads owns a row; a thread holds its values of up to CH chunks of 8 (in registers between the
-// two passes; rows longer than that are read again).  VEC: rows are 16-byte aligned, chunks are loaded whole.
-template <typename T, bool VEC, int NW, int CH>
-__global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW) void quantize_rows_kernel(const T* __restrict__ x, PhRowMap xr, unsigned M,
-                                                                               int K, int8_t* __restrict__ q,
-                                                                               int64_t q_pitch, float* __restrict__ scale) {
-  constexpr int TPR = 64 * NW;
-  const int lane = threadIdx.x & (TPR - 1);
-  const unsigned m = NW == 1 ? blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
-  if (NW == 1 && m >= M) return;
-  const T* row = x + ph_row_off(xr, m);
-  const int step = TPR * 8;
-  float v[CH][8];
-  unsigned am = 0;
-  auto load = [&](int k, float* o) {
-    if (VEC && k + 8 <= K) {
-      const Vec8<T> c = *(const Vec8<T>*)(row + k);
+// round_half_even(x / s), eight values to eight bytes.  x * (1/s) is within 127 * 2^-23 of the quotient, so its rounding
+// is the wanted number or its neighbour; the remainder x - q s is exact in one fused operation and tells which.  Where no
+// remainder reaches half a step, as almost always, all eight stand.
+__device__ __forceinline__ uint64_t quantize8(const float* x, const RowScale& r) {
+  float q[8], worst = 0.f;
 #pragma unroll
-      for (int i = 0; i < 8; i++) o[i] = c.get(i);
-    } else {
+  for (int i = 0; i < 8; i++) {
+    q[i] = rintf(x[i] * r.inv);
+    worst = fmaxf(worst, fabsf(__builtin_fmaf(-q[i], r.s, x[i])));
+  }
+  if (worst >= r.half) {
 #pragma unroll
-      for (int i = 0; i < 8; i++) o[i] = k + i < K ? to_f32(row[k + i]) : 0.f;
-    }
-  };
-#pragma unroll
-  for (int c = 0; c < CH; c++) {
-    const int k = c * step + lane * 8;
-    if (k < K) {
-      load(k, v[c]);
-#pragma unroll
-      for (int i = 0; i < 8; i++) am = max(am, abs_bits(v[c][i]));
+    for (int i = 0; i < 8; i++) {
+      const float rem = __builtin_fmaf(-q[i], r.s, x[i]), a = fabsf(rem);
+      if (a > r.half || (a == r.half && ((int)q[i] & 1))) q[i] += rem > 0.f ? 1.f : -1.f;
     }
   }
-  for (int k = CH * step + lane * 8; k < K; k += step) {
+  unsigned lo = 0, hi = 0;
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    lo |= ((unsigned)(int)q[i] & 255u) << (8 * i);
+    hi |= ((unsigned)(int)q[i + 4] & 255u) << (8 * i);
+  }
+  return r.finite ? ((uint64_t)hi << 32 | lo) : 0;
+}
+
+// eight values from k on, zeros behind the row's end; rows start at any multiple of their element
+template <typename T>
+__device__ __forceinline__ void load8(const T* row, int k, int K, float* o) {
+  typedef T t8 __attribute__((ext_vector_type(8), aligned(sizeof(T))));
+  if (k + 8 <= K) {
+    const t8 c = *(const t8*)(row + k);
+#pragma unroll
+    for (int i = 0; i < 8; i++) o[i] = (float)c[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; i++) o[i] = k + i < K ? (float)row[k + i] : 0.f;
+  }
+}
+
+// G lanes own a row (G <= 64: several rows a wave; more: a block of G threads), with up to CH chunks of 8 values a lane
+// kept in registers between the two passes; what a longer row has beyond is read again.
+template <typename T, int G, int CH>
+__global__ __launch_bounds__(G <= 64 ? 256 : G) void quantize_rows_kernel(const T* __restrict__ x, PhRowMap xr, unsigned M, int K,
+                                                                         int8_t* __restrict__ q, int64_t q_pitch,
+                                                                         float* __restrict__ scale) {
+  constexpr int STEP = G * 8;
+  const int lane = threadIdx.x % G;
+  constexpr int PER = G <= 64 ? 256 / G : 1;   // rows of a block
+  const unsigned m = blockIdx.x * PER + threadIdx.x / G;
+  if (m >= M) return;   // (G > 64: never)
+  const T* row = x + ph_row_off(xr, m);
+  float v[CH][8];
+  unsigned am = 0;
+#pragma unroll
+  for (int c = 0; c < CH; c++) {
+    const int k = c * STEP + lane * 8;
+    if (k < K) {
+      load8(row, k, K, v[c]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; i++) v[c][i] = 0.f;
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < CH; c++)
+#pragma unroll
+    for (int i = 0; i < 8; i++) am = max(am, abs_bits(v[c][i]));
+  for (int k = CH * STEP + lane * 8; k < K; k += STEP) {
     float t[8];
-    load(k, t);
+    load8(row, k, K, t);
 #pragma unroll
     for (int i = 0; i < 8; i++) am = max(am, abs_bits(t[i]));
   }
 #pragma unroll
-  for (int d = 32; d; d >>= 1) am = max(am, (unsigned)__shfl_xor((int)am, d));
-  if (NW > 1) {
-    __shared__ unsigned s_am[NW];
+  for (int d = (G < 64 ? G : 64) / 2; d; d >>= 1) am = max(am, (unsigned)__shfl_xor((int)am, d));
+  if constexpr (G > 64) {
+    __shared__ unsigned s_am[G / 64];
     if ((lane & 63) == 0) s_am[lane >> 6] = am;
     __syncthreads();
-    am = 0;
 #pragma unroll
-    for (int w = 0; w < NW; w++) am = max(am, s_am[w]);
+    for (int w = 0; w < G / 64; w++) am = max(am, s_am[w]);
   }
-  bool finite;
-  const RowScale r = row_scale(am, finite);
-  if (lane == 0) scale[m] = finite ? r.s : __uint_as_float(0x7fc00000u);
-  int8_t* qrow = q + (int64_t)m * q_pitch;
-  auto store = [&](int k, const float* o) {   // (pitch and base are multiples of 16: whole chunks, also the last)
-    union { int8_t b[8]; uint64_t u; } p;
-#pragma unroll
-    for (int i = 0; i < 8; i++) p.b[i] = finite ? (int8_t)quant_one(o[i], r) : (int8_t)0;
-    *(uint64_t*)(qrow + k) = p.u;
-  };
+  const RowScale r = row_scale(am);
+  if (lane == 0) scale[m] = scale_out(r);
+  int8_t* const qrow = q + (int64_t)m * q_pitch;   // (pitch and base are multiples of 16: whole chunks, also the last)
 #pragma unroll
   for (int c = 0; c < CH; c++) {
-    const int k = c * step + lane * 8;
-    if (k < K) store(k, v[c]);
+    const int k = c * STEP + lane * 8;
+    if (k < K) *(uint64_t*)(qrow + k) = quantize8(v[c], r);
   }
-  for (int k = CH * step + lane * 8; k < K; k += step) {
+  for (int k = CH * STEP + lane * 8; k < K; k += STEP) {
     float t[8];
-    load(k, t);
-    store(k, t);
+    load8(row, k, K, t);
+    *(uint64_t*)(qrow + k) = quantize8(t, r);
   }
 }
 
+// As few lanes own a row as hold it in 4 chunks each (120704 rows of 384 bf16: 31 us with 16 lanes a row, 47 with 64 --
+// four rows of a wave are on their way at once, and no lane idles), but more of them where there are few rows (3772 rows:
+// 5.2 us with 16, 4.0 with 64).
 template <typename T>
 static int launch_quantize_t(const T* x, const PhRowMap& xr, unsigned M, int K, int8_t* q, int64_t pitch, float* scale,
                              hipStream_t st) {
-  const int64_t strides = xr.flat ? xr.s2 : (xr.s0 | xr.s1 | xr.s2);
-  const bool vec = ((uintptr_t)x & 15) == 0 && (strides * (int64_t)sizeof(T)) % 16 == 0;
-  const bool wave = K <= 2048;   // a wave holds 4 chunks of 512 values
-#define PH_Q(V, NW, CH)                                                                                         \
-  hipLaunchKernelGGL((quantize_rows_kernel<T, V, NW, CH>), dim3(NW == 1 ? (M + 3) / 4 : M), dim3(NW == 1 ? 256 : 64 * NW), 0, \
-                     st, x, xr, M, K, q, pitch, scale)
-  if (wave) {
-    if (vec) { if (K <= 512) PH_Q(true, 1, 1); else PH_Q(true, 1, 4); }
-    else { if (K <= 512) PH_Q(false, 1, 1); else PH_Q(false, 1, 4); }
-  } else {
-    if (vec) PH_Q(true, 8, 2); else PH_Q(false, 8, 2);
+  static const int groups[] = {8, 16, 32, 64, 256, 1024};
+  int g = 0;
+  while (g < 5 && groups[g] * 32 < K) g++;
+  while (g < 5 && groups[g] * 8 < K && (int64_t)M * groups[g] < 64 * 4096) g++;
+#define PH_Q(G)                                                                                                            \
+  hipLaunchKernelGGL((quantize_rows_kernel<T, G, 4>), dim3(G <= 64 ? (M - 1) / (G <= 64 ? 256 / G : 1) + 1 : M),              \
+                     dim3(G <= 64 ? 256 : G), 0, st, x, xr, M, K, q, pitch, scale);                                         \
+  break
+  switch (g) {
+    case 0: PH_Q(8);
+    case 1: PH_Q(16);
+    case 2: PH_Q(32);
+    case 3: PH_Q(64);
+    case 4: PH_Q(256);
+    default: PH_Q(1024);
   }
 #undef PH_Q
   PH_CHECK(hipGetLastError());
@@ -471,20 +476,7 @@ static int launch_tile(const PhW8Params& p, int parts, hipStream_t st) {
 struct FloatRows {
   const void* x;
   PhRowMap r;
-  int vec;   // rows are 16-byte aligned
 };
-
-template <typename T>
-__device__ __forceinline__ void load8(const T* row, int k, int K, bool vec, float* o) {
-  if (vec && k + 8 <= K) {
-    const Vec8<T> c = *(const Vec8<T>*)(row + k);
-#pragma unroll
-    for (int i = 0; i < 8; i++) o[i] = c.get(i);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; i++) o[i] = k + i < K ? to_f32(row[k + i]) : 0.f;
-  }
-}
 
 // M <= 8 rows -> int8 rows of `pitch` bytes and their scales in LDS; W waves, W / (M rounded up to a power of two) a row
 template <int W, typename T>
@@ -502,7 +494,7 @@ __device__ __forceinline__ void quantize_block(const FloatRows& f, unsigned M, i
   if (has) {
     for (int k = k0; k < K; k += step) {
       float v[8];
-      load8(xr, k, K, f.vec, v);
+      load8(xr, k, K, v);
 #pragma unroll
       for (int i = 0; i < 8; i++) {
         am = max(am, abs_bits(v[i]));
@@ -517,21 +509,17 @@ __device__ __forceinline__ void quantize_block(const FloatRows& f, unsigned M, i
   if (has) {
     am = 0;
     for (unsigned w = 0; w < per; w++) am = max(am, amax[row * per + w]);
-    bool finite;
-    const RowScale r = row_scale(am, finite);
-    if (lane == 0 && wave % per == 0) scale[row] = finite ? r.s : __uint_as_float(0x7fc00000u);
+    const RowScale r = row_scale(am);
+    if (lane == 0 && wave % per == 0) scale[row] = scale_out(r);
     for (int k = k0; k < K; k += step) {
       float v[8];
       if (k == k0) {
 #pragma unroll
         for (int i = 0; i < 8; i++) v[i] = first[i];
       } else {
-        load8(xr, k, K, f.vec, v);
+        load8(xr, k, K, v);
       }
-      union { int8_t b[8]; uint64_t u; } o;
-#pragma unroll
-      for (int i = 0; i < 8; i++) o.b[i] = finite ? (int8_t)quant_one(v[i], r) : (int8_t)0;
-      *(uint64_t*)(q + (int)row * pitch + k) = o.u;
+      *(uint64_t*)(q + (int)row * pitch + k) = quantize8(v, r);
     }
   }
   __syncthreads();
@@ -656,8 +644,9 @@ static Choice choose(int64_t M, int N, int nkb) {
   auto join = [&](int parts) { return parts > 1 ? 3.3f + (float)M * n16 * 4e-6f * parts / 2.f : 0.f; };   // (2 TB/s)
   Choice best = {K_64, 1};
   float least = 1e30f;
+  const int64_t small = (M + 63) / 64 * ((N + 63) / 64);   // blocks of the smallest tile: two rounds of them need no parts
   for (int parts = 1; parts <= 32 && parts <= steps; parts *= 2) {
-    if (parts > 1 && (float)M * n16 * parts > (float)(1 << 24)) break;
+    if (parts > 1 && (small >= 1024 || (float)M * n16 * parts > (float)(1 << 24))) break;
     const int s = (steps + parts - 1) / parts;
     for (int k = 0; k < N_KERNELS; k++) {
       const Kernel& c = kernels[k];
@@ -678,8 +667,7 @@ static Choice choose(int64_t M, int N, int nkb) {
   return best;
 }
 
-static int64_t parts_bytes(int64_t M, int N, int nkb) {
-  const Choice c = choose(M, N, nkb);
+static int64_t parts_bytes(const Choice& c, int64_t M, int N) {
   return c.parts > 1 ? (int64_t)c.parts * M * ((N + 15) / 16 * 16) * 4 : 0;
 }
 
@@ -701,8 +689,7 @@ static int launch_kernel(const PhW8Params& p, const Choice& c, hipStream_t st) {
 
 // parts_bytes() of workspace at p.parts
 template <typename O>
-static int launch_product_t(const PhW8Params& p, hipStream_t st) {
-  const Choice c = choose(p.M, p.N, p.nkb);
+static int launch_product_t(const PhW8Params& p, const Choice& c, hipStream_t st) {
   if (c.parts == 1) return launch_kernel<false, O>(p, c, st);
   if (launch_kernel<true, O>(p, c, st)) return -1;
   const int64_t pieces = (int64_t)p.M * ((p.N + 3) / 4);
@@ -730,11 +717,11 @@ static int launch_few_float(const PhW8Params& p, int x_type, const FloatRows& f,
   }
 }
 
-static int launch_product(const PhW8Params& p, int out_type, hipStream_t st) {
+static int launch_product(const PhW8Params& p, const Choice& c, int out_type, hipStream_t st) {
   switch (out_type) {
-    case PH_F32: return launch_product_t<float>(p, st);
-    case PH_F16: return launch_product_t<_Float16>(p, st);
-    default: return launch_product_t<bf16>(p, st);
+    case PH_F32: return launch_product_t<float>(p, c, st);
+    case PH_F16: return launch_product_t<_Float16>(p, c, st);
+    default: return launch_product_t<bf16>(p, c, st);
   }
 }
 
@@ -824,8 +811,8 @@ bool some(const char* who, const void* a, const void* b) {
   return false;
 }
 
-bool aligned16(const void* p, const PhRowMap& r, int64_t elem) {
-  return ((uintptr_t)p & 15) == 0 && ((r.s0 | r.s1 | r.s2) * elem) % 16 == 0;
+bool aligned16(const void* p, const PhRowMap& r) {   // rows of bytes
+  return ((uintptr_t)p & 15) == 0 && (r.s0 | r.s1 | r.s2) % 16 == 0;
 }
 
 int quantize(const void* x, int type, const PhRowMap& xr, unsigned M, int K, int8_t* q, int64_t pitch, float* scale,
@@ -861,6 +848,31 @@ struct Pieces {
     used += up(n * (int64_t)sizeof(T), 256);
     return p;
   }
+};
+
+// The workspace of one product: its parts' sums, 8-bit rows and their scales, as far as the call needs them.
+struct RowsSpace {
+  Pieces w;
+  Choice choice;
+  int* parts;
+  int8_t* q = nullptr;
+  float* s = nullptr;
+  RowsSpace(void* ws, int64_t M, int K, int N, bool rows, bool scales) : w{(char*)ws}, choice(choose(M, N, nkb_of(K))) {
+    parts = (int*)w.take<char>(parts_bytes(choice, M, N));
+    if (rows) q = w.take<int8_t>(M * q_pitch_of(K));
+    if (scales) s = w.take<float>(M);
+  }
+  int64_t used() const { return w.used; }
+};
+// Of two layers: the inner rows in f32, and the larger of the two products' spaces, one after the other in one place.
+struct PairSpace {
+  float* h;
+  RowsSpace a, b;
+  int64_t hbytes;
+  PairSpace(void* ws, int64_t M, int K, int H, int N)
+      : h((float*)ws), a((char*)ws + up(M * up(H, 4) * 4, 256), M, K, H, true, true),
+        b((char*)ws + up(M * up(H, 4) * 4, 256), M, H, N, true, true), hbytes(up(M * up(H, 4) * 4, 256)) {}
+  int64_t used() const { return hbytes + (a.used() > b.used() ? a.used() : b.used()); }
 };
 
 }  // namespace
@@ -911,40 +923,20 @@ int64_t ph_w8_workspace(int op, int64_t m, int k, int h, int n) {
     return -1;
   }
   if (m == 0) return 0;
-  Pieces w = {nullptr};
   switch (op) {
-    case PH_W8_MATMUL:
-      w.take<char>(parts_bytes(m, n, nkb_of(k)));
-      break;
-    case PH_W8_MATMUL_ANY:   // rows that are not 16-byte aligned are laid out anew
-      w.take<char>(parts_bytes(m, n, nkb_of(k)));
-      w.take<int8_t>(m * q_pitch_of(k));
-      break;
-    case PH_W8_LINEAR:
-      if (few_float(m, k)) break;
-      w.take<char>(parts_bytes(m, n, nkb_of(k)));
-      w.take<int8_t>(m * q_pitch_of(k));
-      w.take<float>(m);
-      break;
-    case PH_W8_FEED_FORWARD: {
+    case PH_W8_MATMUL: return RowsSpace(nullptr, m, k, n, false, false).used();
+    case PH_W8_MATMUL_ANY: return RowsSpace(nullptr, m, k, n, true, false).used();
+    case PH_W8_LINEAR: return few_float(m, k) ? 0 : RowsSpace(nullptr, m, k, n, true, true).used();
+    case PH_W8_FEED_FORWARD:
       if (h < 1) {
         ph_set_error("ph_w8_workspace: a feed-forward's inner width is 1 or more");
         return -1;
       }
-      const int64_t a = parts_bytes(m, h, nkb_of(k)), b = parts_bytes(m, n, nkb_of(h));
-      w.take<char>(a > b ? a : b);   // (the two products run one after the other)
-      w.take<int8_t>(m * q_pitch_of(k));
-      w.take<float>(m);
-      w.take<float>(m * up(h, 4));
-      w.take<int8_t>(m * q_pitch_of(h));
-      w.take<float>(m);
-      break;
-    }
+      return PairSpace(nullptr, m, k, h, n).used();
     default:
       ph_set_error("ph_w8_workspace: unknown operator %d", op);
       return -1;
   }
-  return w.used;
 }
 
 static bool ws_ok(const char* who, const void* ws, int64_t have, int64_t need) {
@@ -963,21 +955,20 @@ int ph_w8_matmul(int device, void* stream, const int8_t* q, const ph_rows* rows,
   ph_rows orow = *rows;
   for (int d = 0; d < 3; d++) orow.stride[d] = out_stride[d];
   PhRowMap qr = row_map(*rows);
-  const bool direct = aligned16(q, qr, 1);
-  if (!ws_ok(who, ws, ws_bytes, ph_w8_workspace(direct ? PH_W8_MATMUL : PH_W8_MATMUL_ANY, M, layer->k, 0, layer->n))) return -3;
+  const bool direct = aligned16(q, qr);
+  const RowsSpace w(ws, M, layer->k, layer->n, !direct, false);
+  if (!ws_ok(who, ws, ws_bytes, w.used())) return -3;
   W8_DEVICE(device);
-  Pieces w = {(char*)ws};
-  int* parts = (int*)w.take<char>(parts_bytes(M, layer->n, nkb_of(layer->k)));
   if (!direct) {
     const int64_t pitch = q_pitch_of(layer->k), pieces = M * (pitch / 16);
-    int8_t* even = w.take<int8_t>(M * pitch);
     hipLaunchKernelGGL(repitch_kernel, dim3((unsigned)((pieces + 255) / 256)), dim3(256), 0, (hipStream_t)stream, q, qr,
-                       (unsigned)M, layer->k, even, pitch);
+                       (unsigned)M, layer->k, w.q, pitch);
     PH_CHECK(hipGetLastError());
-    q = even;
+    q = w.q;
     qr = even_rows(pitch);
   }
-  return launch_product(product_params(q, qr, scale, (unsigned)M, *layer, out, row_map(orow), parts), out_type, (hipStream_t)stream);
+  return launch_product(product_params(q, qr, scale, (unsigned)M, *layer, out, row_map(orow), w.parts), w.choice, out_type,
+                        (hipStream_t)stream);
 }
 
 int ph_w8_linear(int device, void* stream, const void* x, int x_type, const ph_rows* rows, const ph_w8_layer* layer, void* out,
@@ -987,14 +978,13 @@ int ph_w8_linear(int device, void* stream, const void* x, int x_type, const ph_r
   if (!rows_ok(who, rows, M) || !layer_ok(who, layer) || !type_ok(who, x_type) || !type_ok(who, out_type)) return -1;
   if (M == 0) return 0;
   if (!some(who, x, out) || !some(who, out, out_stride)) return -1;
-  if (!ws_ok(who, ws, ws_bytes, ph_w8_workspace(PH_W8_LINEAR, M, layer->k, 0, layer->n))) return -3;
   ph_rows orow = *rows;
   for (int d = 0; d < 3; d++) orow.stride[d] = out_stride[d];
-  W8_DEVICE(device);
   hipStream_t st = (hipStream_t)stream;
   const PhRowMap xr = row_map(*rows), outr = row_map(orow);
   if (few_float(M, layer->k)) {
-    const FloatRows f = {x, xr, aligned16(x, xr, x_type == PH_F32 ? 4 : 2)};
+    W8_DEVICE(device);
+    const FloatRows f = {x, xr};
     const PhW8Params p = product_params(nullptr, xr, nullptr, (unsigned)M, *layer, out, outr, nullptr);
     switch (out_type) {
       case PH_F32: return launch_few_float<float>(p, x_type, f, st);
@@ -1003,12 +993,11 @@ int ph_w8_linear(int device, void* stream, const void* x, int x_type, const ph_r
     }
   }
   const int64_t pitch = q_pitch_of(layer->k);
-  Pieces w = {(char*)ws};
-  int* parts = (int*)w.take<char>(parts_bytes(M, layer->n, nkb_of(layer->k)));
-  int8_t* q = w.take<int8_t>(M * pitch);
-  float* s = w.take<float>(M);
-  if (quantize(x, x_type, xr, (unsigned)M, layer->k, q, pitch, s, st)) return -1;
-  return launch_product(product_params(q, even_rows(pitch), s, (unsigned)M, *layer, out, outr, parts), out_type, st);
+  const RowsSpace w(ws, M, layer->k, layer->n, true, true);
+  if (!ws_ok(who, ws, ws_bytes, w.used())) return -3;
+  W8_DEVICE(device);
+  if (quantize(x, x_type, xr, (unsigned)M, layer->k, w.q, pitch, w.s, st)) return -1;
+  return launch_product(product_params(w.q, even_rows(pitch), w.s, (unsigned)M, *layer, out, outr, w.parts), w.choice, out_type, st);
 }
 
 int ph_w8_feed_forward(int device, void* stream, const void* x, int x_type, const ph_rows* rows, const ph_w8_layer* layer1,
@@ -1023,25 +1012,20 @@ int ph_w8_feed_forward(int device, void* stream, const void* x, int x_type, cons
   }
   if (M == 0) return 0;
   if (!some(who, x, out) || !some(who, out, out_stride)) return -1;
-  if (!ws_ok(who, ws, ws_bytes, ph_w8_workspace(PH_W8_FEED_FORWARD, M, layer1->k, layer1->n, layer2->n))) return -3;
+  const int K = layer1->k, H = layer1->n;
+  const PairSpace w(ws, M, K, H, layer2->n);
+  if (!ws_ok(who, ws, ws_bytes, w.used())) return -3;
   ph_rows orow = *rows;
   for (int d = 0; d < 3; d++) orow.stride[d] = out_stride[d];
   W8_DEVICE(device);
   hipStream_t st = (hipStream_t)stream;
-  const int K = layer1->k, H = layer1->n;
   const int64_t pitch = q_pitch_of(K), hpitch = up(H, 4), pitch2 = q_pitch_of(H);
-  Pieces w = {(char*)ws};
-  const int64_t pa = parts_bytes(M, H, nkb_of(K)), pb = parts_bytes(M, layer2->n, nkb_of(H));
-  int* parts = (int*)w.take<char>(pa > pb ? pa : pb);
-  int8_t* q = w.take<int8_t>(M * pitch);
-  float* s = w.take<float>(M);
-  float* h = w.take<float>(M * hpitch);
-  int8_t* q2 = w.take<int8_t>(M * pitch2);
-  float* s2 = w.take<float>(M);
-  if (quantize(x, x_type, row_map(*rows), (unsigned)M, K, q, pitch, s, st)) return -1;
-  if (launch_product(product_params(q, even_rows(pitch), s, (unsigned)M, *layer1, h, even_rows(hpitch), parts), PH_F32, st)) return -1;
-  if (quantize(h, PH_F32, even_rows(hpitch), (unsigned)M, H, q2, pitch2, s2, st)) return -1;
-  return launch_product(product_params(q2, even_rows(pitch2), s2, (unsigned)M, *layer2, out, row_map(orow), parts), out_type, st);
+  if (quantize(x, x_type, row_map(*rows), (unsigned)M, K, w.a.q, pitch, w.a.s, st)) return -1;
+  if (launch_product(product_params(w.a.q, even_rows(pitch), w.a.s, (unsigned)M, *layer1, w.h, even_rows(hpitch), w.a.parts),
+                     w.a.choice, PH_F32, st)) return -1;
+  if (quantize(w.h, PH_F32, even_rows(hpitch), (unsigned)M, H, w.b.q, pitch2, w.b.s, st)) return -1;
+  return launch_product(product_params(w.b.q, even_rows(pitch2), w.b.s, (unsigned)M, *layer2, out, row_map(orow), w.b.parts),
+                        w.b.choice, out_type, st);
 }
 
 }  // extern "C"
