@@ -29,6 +29,7 @@ struct PhW8Params {
   const float* bias;     // [N16] or NULL
   const float* slope;    // [N16] or NULL
   int act;
+  int stream;            // store past the caches
   unsigned M;
   int N, K, nkb, nnb;    // nkb = K128 / 64 fragments along K (even), nnb = N16 / 16 along N
   void* out;

@@ -12,62 +12,106 @@
 
 // ---- quantisation of rows ------------------------------------------------------------------------------------------
 
-// |v| as an integer that orders like it; NaN and infinities are >= 0x7f800000
-__device__ __forceinline__ unsigned abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+// Running maximum of magnitudes that a NaN stays in (fmaxf would drop it).
+__device__ __forceinline__ float max_abs(float m, float v) { return __builtin_elementwise_maximum(m, fabsf(v)); }
+// Over groups of G lanes side by side (G = 8 .. 64); all get it.
+template <int CTRL>
+__device__ __forceinline__ float max_dpp(float m) {
+  return __builtin_elementwise_maximum(m, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(m), CTRL, 0xf, 0xf, true)));
+}
+__device__ __forceinline__ float max_16(float m) {   // lanes 16 apart
+  const auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(m), __float_as_uint(m), false, false);
+  return __builtin_elementwise_maximum(__uint_as_float(p[0]), __uint_as_float(p[1]));
+}
+__device__ __forceinline__ float max_32(float m) {   // lanes 32 apart
+  const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(m), __float_as_uint(m), false, false);
+  return __builtin_elementwise_maximum(__uint_as_float(p[0]), __uint_as_float(p[1]));
+}
+template <int G>
+__device__ __forceinline__ float max_group(float m) {
+  m = max_dpp<0xb1>(m);    // lanes 1 apart
+  m = max_dpp<0x4e>(m);    // 2 apart
+  m = max_dpp<0x141>(m);   // 4: a half row mirrored, its quads being alike
+  if (G > 8) m = max_dpp<0x140>(m);   // 8: a row mirrored
+  if (G > 16) m = max_16(m);
+  if (G > 32) m = max_32(m);
+  return m;
+}
 
 struct RowScale {
   float s, inv, half;   // scale, 1 / scale, scale / 2
   bool finite;
 };
-__device__ __forceinline__ RowScale row_scale(unsigned amax_bits) {
+__device__ __forceinline__ RowScale row_scale(float amax) {
   RowScale r;
-  r.finite = amax_bits < 0x7f800000u;
-  r.s = r.finite ? fmaxf(__uint_as_float(amax_bits) / 127.f, 0x1p-126f) : 1.f;
+  r.finite = amax < __builtin_inff();
+  r.s = r.finite ? fmaxf(amax / 127.f, 0x1p-126f) : 1.f;
   r.inv = 1.f / r.s;
   r.half = 0.5f * r.s;
   return r;
 }
-__device__ __forceinline__ float scale_out(const RowScale& r) { return r.finite ? r.s : __uint_as_float(0x7fc00000u); }
+__device__ __forceinline__ float scale_out(const RowScale& r) { return r.finite ? r.s : __builtin_nanf(""); }
 
-// round_half_even(x / s), eight values to eight bytes.  x * (1/s) is within 127 * 2^-23 of the quotient, so its rounding
-// is the wanted number or its neighbour; the remainder x - q s is exact in one fused operation and tells which.  Where no
-// remainder reaches half a step, as almost always, all eight stand.
-__device__ __forceinline__ uint64_t quantize8(const float* x, const RowScale& r) {
-  float q[8], worst = 0.f;
+// round_half_even(x / s), N values to N bytes.  Adding 1.5 * 2^23 rounds to a whole number, which then stands in the low
+// bits of the sum.  x * (1/s) is within 127 * 2^-23 of the quotient, so that number is the wanted one or its neighbour;
+// the remainder x - q s is exact in one fused operation and tells which.  Where no remainder reaches half a step, as
+// almost always, all stand.
+template <int N>
+__device__ __forceinline__ void quantize_n(const float (&x)[N], const RowScale& r, unsigned (&out)[N / 4]) {
+  constexpr float MAGIC = 12582912.f;
+  float t[N], worst = 0.f;
 #pragma unroll
-  for (int i = 0; i < 8; i++) {
-    q[i] = rintf(x[i] * r.inv);
-    worst = fmaxf(worst, fabsf(__builtin_fmaf(-q[i], r.s, x[i])));
+  for (int i = 0; i < N; i++) {
+    t[i] = __builtin_fmaf(x[i], r.inv, MAGIC);
+    worst = fmaxf(worst, fabsf(__builtin_fmaf(-(t[i] - MAGIC), r.s, x[i])));
   }
   if (worst >= r.half) {
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-      const float rem = __builtin_fmaf(-q[i], r.s, x[i]), a = fabsf(rem);
-      if (a > r.half || (a == r.half && ((int)q[i] & 1))) q[i] += rem > 0.f ? 1.f : -1.f;
+    for (int i = 0; i < N; i++) {
+      const float rem = __builtin_fmaf(-(t[i] - MAGIC), r.s, x[i]), a = fabsf(rem);
+      const bool odd = __float_as_uint(t[i]) & 1;
+      const float far = odd ? a : __uint_as_float(__float_as_uint(a) - (a > 0.f));   // a tie moves an odd number only
+      t[i] += far >= r.half ? __builtin_copysignf(1.f, rem) : 0.f;
     }
   }
-  unsigned lo = 0, hi = 0;
 #pragma unroll
-  for (int i = 0; i < 4; i++) {
-    lo |= ((unsigned)(int)q[i] & 255u) << (8 * i);
-    hi |= ((unsigned)(int)q[i + 4] & 255u) << (8 * i);
+  for (int i = 0; i < N / 4; i++) {
+    const unsigned lo = __builtin_amdgcn_perm(__float_as_uint(t[4 * i + 1]), __float_as_uint(t[4 * i]), 0x0c0c0400u);
+    const unsigned hi = __builtin_amdgcn_perm(__float_as_uint(t[4 * i + 3]), __float_as_uint(t[4 * i + 2]), 0x04000c0cu);
+    out[i] = r.finite ? lo | hi : 0;
   }
-  return r.finite ? ((uint64_t)hi << 32 | lo) : 0;
 }
 
-// eight values from k on, zeros behind the row's end; rows start at any multiple of their element
+// Eight values of a row from k on; rows start at any multiple of their element.  Where fewer are left, the row's last
+// eight: a value seen twice does not change a maximum, and the bytes move to their place by `shift` bits.
 template <typename T>
-__device__ __forceinline__ void load8(const T* row, int k, int K, float* o) {
+struct Eight {
+  T v __attribute__((ext_vector_type(8)));
   typedef T t8 __attribute__((ext_vector_type(8), aligned(sizeof(T))));
-  if (k + 8 <= K) {
-    const t8 c = *(const t8*)(row + k);
+  __device__ __forceinline__ void load_long(const T* row, int k, int K) { v = *(const t8*)(row + min(k, K - 8)); }   // K >= 8
+  __device__ __forceinline__ void load(const T* row, int k, int K) {
+    if (K >= 8) {
+      load_long(row, k, K);
+    } else {
 #pragma unroll
-    for (int i = 0; i < 8; i++) o[i] = (float)c[i];
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; i++) o[i] = k + i < K ? (float)row[k + i] : 0.f;
+      for (int i = 0; i < 8; i++) v[i] = i < K ? row[i] : (T)0.f;
+    }
   }
-}
+  static __device__ __forceinline__ int shift(int k, int K) { return 8 * max(0, k - max(K - 8, 0)); }   // k < K
+  __device__ __forceinline__ float max_with(float m) const {
+#pragma unroll
+    for (int i = 0; i < 8; i++) m = max_abs(m, (float)v[i]);
+    return m;
+  }
+  __device__ __forceinline__ uint64_t quantize(const RowScale& r) const {
+    float x[8];
+    unsigned o[2];
+#pragma unroll
+    for (int i = 0; i < 8; i++) x[i] = (float)v[i];
+    quantize_n(x, r, o);
+    return (uint64_t)o[1] << 32 | o[0];
+  }
+};
 
 // G lanes own a row (G <= 64: several rows a wave; more: a block of G threads), with up to CH chunks of 8 values a lane
 // kept in registers between the two passes; what a longer row has beyond is read again.
@@ -81,36 +125,26 @@ __global__ __launch_bounds__(G <= 64 ? 256 : G) void quantize_rows_kernel(const 
   const unsigned m = blockIdx.x * PER + threadIdx.x / G;
   if (m >= M) return;   // (G > 64: never)
   const T* row = x + ph_row_off(xr, m);
-  float v[CH][8];
-  unsigned am = 0;
-#pragma unroll
-  for (int c = 0; c < CH; c++) {
-    const int k = c * STEP + lane * 8;
-    if (k < K) {
-      load8(row, k, K, v[c]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; i++) v[c][i] = 0.f;
-    }
-  }
+  Eight<T> v[CH];
+  float am = 0.f;
 #pragma unroll
   for (int c = 0; c < CH; c++)
+    if (c * STEP < K) v[c].load(row, c * STEP + lane * 8, K);
 #pragma unroll
-    for (int i = 0; i < 8; i++) am = max(am, abs_bits(v[c][i]));
+  for (int c = 0; c < CH; c++)
+    if (c * STEP < K) am = v[c].max_with(am);
   for (int k = CH * STEP + lane * 8; k < K; k += STEP) {
-    float t[8];
-    load8(row, k, K, t);
-#pragma unroll
-    for (int i = 0; i < 8; i++) am = max(am, abs_bits(t[i]));
+    Eight<T> t;
+    t.load(row, k, K);
+    am = t.max_with(am);
   }
-#pragma unroll
-  for (int d = (G < 64 ? G : 64) / 2; d; d >>= 1) am = max(am, (unsigned)__shfl_xor((int)am, d));
+  am = max_group<(G < 64 ? G : 64)>(am);
   if constexpr (G > 64) {
-    __shared__ unsigned s_am[G / 64];
+    __shared__ float s_am[G / 64];
     if ((lane & 63) == 0) s_am[lane >> 6] = am;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < G / 64; w++) am = max(am, s_am[w]);
+    for (int w = 0; w < G / 64; w++) am = max_abs(am, s_am[w]);
   }
   const RowScale r = row_scale(am);
   if (lane == 0) scale[m] = scale_out(r);
@@ -118,18 +152,18 @@ __global__ __launch_bounds__(G <= 64 ? 256 : G) void quantize_rows_kernel(const 
 #pragma unroll
   for (int c = 0; c < CH; c++) {
     const int k = c * STEP + lane * 8;
-    if (k < K) *(uint64_t*)(qrow + k) = quantize8(v[c], r);
+    if (k < K) *(uint64_t*)(qrow + k) = v[c].quantize(r) >> Eight<T>::shift(k, K);
   }
   for (int k = CH * STEP + lane * 8; k < K; k += STEP) {
-    float t[8];
-    load8(row, k, K, t);
-    *(uint64_t*)(qrow + k) = quantize8(t, r);
+    Eight<T> t;
+    t.load(row, k, K);
+    *(uint64_t*)(qrow + k) = t.quantize(r) >> Eight<T>::shift(k, K);
   }
 }
 
-// As few lanes own a row as hold it in 4 chunks each (120704 rows of 384 bf16: 31 us with 16 lanes a row, 47 with 64 --
-// four rows of a wave are on their way at once, and no lane idles), but more of them where there are few rows (3772 rows:
-// 5.2 us with 16, 4.0 with 64).
+// As few lanes own a row as hold it in 4 chunks each (120704 rows of 384 bf16: 28 us = 5.0 TB/s with 16 lanes a row, 47 with
+// 64 -- four rows of a wave are on their way at once, and no lane idles), but more of them where there are few rows (3772
+// rows: 5.2 us with 16, 3.8 with 64).
 template <typename T>
 static int launch_quantize_t(const T* x, const PhRowMap& xr, unsigned M, int K, int8_t* q, int64_t pitch, float* scale,
                              hipStream_t st) {
@@ -232,8 +266,7 @@ __device__ __forceinline__ f32x4 w8_values(const i32x4 acc, const Channels& c, f
 
 // one sum of four channels -> out
 template <typename O>
-__device__ __forceinline__ void w8_finish4(const PhW8Params& p, const i32x4 a, unsigned m, int n, float s) {
-  const Channels c = w8_channels(p, n);
+__device__ __forceinline__ void w8_finish4(const PhW8Params& p, const i32x4 a, const Channels& c, unsigned m, int n, float s) {
   f32x4 v;
   if (p.act == PH_ACT_RELU) v = w8_values<PH_ACT_RELU>(a, c, s);
   else if (p.act == PH_ACT_PRELU) v = w8_values<PH_ACT_PRELU>(a, c, s);
@@ -254,7 +287,7 @@ struct WaveOut {
   typedef O oe __attribute__((ext_vector_type(16 / sizeof(O)), aligned(sizeof(O))));
   typedef O o4 __attribute__((ext_vector_type(4)));
 
-  template <int ACT>
+  template <int ACT, bool STREAM>
   static __device__ __forceinline__ void put(const PhW8Params& p, const i32x4 (&acc)[TN][TM], unsigned m0, int n0, char* buf,
                                              int lane) {
     const int fr = lane & 15, fq = lane >> 4;
@@ -289,7 +322,10 @@ struct WaveOut {
         if ((UNITS % 64 == 0 || u < UNITS) && m < p.M && n < p.N) {
           const oe w = *(const oe __attribute__((aligned(16)))*)(buf + t * PITCH + col * (int)sizeof(O));
           O* const o = (O*)p.out + ph_row_off(p.outr, m) + n;
-          if (n + PER <= p.N) *(oe*)o = w;
+          if (n + PER <= p.N) {
+            if constexpr (STREAM) __builtin_nontemporal_store(w, (oe*)o);
+            else *(oe*)o = w;
+          }
           else {
 #pragma unroll
             for (int e = 0; e < PER - 1; e++)
@@ -303,9 +339,15 @@ struct WaveOut {
   }
   static __device__ __forceinline__ void store(const PhW8Params& p, const i32x4 (&acc)[TN][TM], unsigned m0, int n0, char* buf,
                                                int lane) {
-    if (p.act == PH_ACT_RELU) put<PH_ACT_RELU>(p, acc, m0, n0, buf, lane);
-    else if (p.act == PH_ACT_PRELU) put<PH_ACT_PRELU>(p, acc, m0, n0, buf, lane);
-    else put<PH_ACT_NONE>(p, acc, m0, n0, buf, lane);
+    if (p.stream) store_act<true>(p, acc, m0, n0, buf, lane);
+    else store_act<false>(p, acc, m0, n0, buf, lane);
+  }
+  template <bool STREAM>
+  static __device__ __forceinline__ void store_act(const PhW8Params& p, const i32x4 (&acc)[TN][TM], unsigned m0, int n0, char* buf,
+                                                   int lane) {
+    if (p.act == PH_ACT_RELU) put<PH_ACT_RELU, STREAM>(p, acc, m0, n0, buf, lane);
+    else if (p.act == PH_ACT_PRELU) put<PH_ACT_PRELU, STREAM>(p, acc, m0, n0, buf, lane);
+    else put<PH_ACT_NONE, STREAM>(p, acc, m0, n0, buf, lane);
   }
 };
 
@@ -481,7 +523,7 @@ struct FloatRows {
 // M <= 8 rows -> int8 rows of `pitch` bytes and their scales in LDS; W waves, W / (M rounded up to a power of two) a row
 template <int W, typename T>
 __device__ __forceinline__ void quantize_block(const FloatRows& f, unsigned M, int K, char* q, int pitch, float* scale,
-                                               unsigned* amax, int wave, int lane) {
+                                               float* amax, int wave, int lane) {
   const T* const x = (const T*)f.x;
   const unsigned per = M > 4 ? 1 : M > 2 ? 2 : M > 1 ? 4 : 8;   // waves of a row (W = 8)
   static_assert(W == 8, "waves are dealt to rows for 8");
@@ -489,37 +531,30 @@ __device__ __forceinline__ void quantize_block(const FloatRows& f, unsigned M, i
   const bool has = row < M;
   const T* const xr = x + ph_row_off(f.r, has ? row : 0);
   const int k0 = ((wave % per) * 64 + lane) * 8, step = per * 512;
-  float first[8];
-  unsigned am = 0;
+  Eight<T> first;
+  float am = 0.f;
   if (has) {
-    for (int k = k0; k < K; k += step) {
-      float v[8];
-      load8(xr, k, K, v);
-#pragma unroll
-      for (int i = 0; i < 8; i++) {
-        am = max(am, abs_bits(v[i]));
-        if (k == k0) first[i] = v[i];
-      }
+    first.load(xr, k0, K);
+    am = first.max_with(am);
+    for (int k = k0 + step; k < K; k += step) {
+      Eight<T> v;
+      v.load(xr, k, K);
+      am = v.max_with(am);
     }
   }
-#pragma unroll
-  for (int d = 32; d; d >>= 1) am = max(am, (unsigned)__shfl_xor((int)am, d));
+  am = max_group<64>(am);
   if (lane == 0) amax[wave] = am;
   __syncthreads();
   if (has) {
-    am = 0;
-    for (unsigned w = 0; w < per; w++) am = max(am, amax[row * per + w]);
+    am = 0.f;
+    for (unsigned w = 0; w < per; w++) am = max_abs(am, amax[row * per + w]);
     const RowScale r = row_scale(am);
     if (lane == 0 && wave % per == 0) scale[row] = scale_out(r);
-    for (int k = k0; k < K; k += step) {
-      float v[8];
-      if (k == k0) {
-#pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = first[i];
-      } else {
-        load8(xr, k, K, v);
-      }
-      *(uint64_t*)(q + (int)row * pitch + k) = quantize8(v, r);
+    if (k0 < K) *(uint64_t*)(q + (int)row * pitch + k0) = first.quantize(r) >> Eight<T>::shift(k0, K);
+    for (int k = k0 + step; k < K; k += step) {
+      Eight<T> v;
+      v.load(xr, k, K);
+      *(uint64_t*)(q + (int)row * pitch + k) = v.quantize(r) >> Eight<T>::shift(k, K);
     }
   }
   __syncthreads();
@@ -532,7 +567,7 @@ __global__ __launch_bounds__(64 * W) void w8_few_kernel(const PhW8Params p, cons
   __shared__ __attribute__((aligned(16))) int red[W][TM][256];
   extern __shared__ __attribute__((aligned(16))) char s_q[];   // FLOAT: the rows in 8 bits
   __shared__ float s_scale[8];
-  __shared__ unsigned s_amax[W];
+  __shared__ float s_amax[W];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int fr = lane & 15, fq = lane >> 4;
   const int nb = blockIdx.x;
@@ -586,7 +621,7 @@ __global__ __launch_bounds__(64 * W) void w8_few_kernel(const PhW8Params p, cons
     const int n = nb * 16 + fq * 4;
     if (m >= p.M || n >= p.N) return;
     if (SPLIT) *(i32x4*)(p.parts + ((int64_t)blockIdx.y * p.M + m) * (p.nnb * 16) + n) = a;
-    else w8_finish4<O>(p, a, m, n, FLOAT ? s_scale[m & 7] : p.qs[m]);
+    else w8_finish4<O>(p, a, w8_channels(p, n), m, n, FLOAT ? s_scale[m & 7] : p.qs[m]);
   }
 }
 
@@ -608,7 +643,7 @@ __global__ __launch_bounds__(256) void w8_join_kernel(const PhW8Params p, int pa
 #pragma unroll
     for (int s = 0; s < 8; s++) a += b[s];
   }
-  w8_finish4<O>(p, a, m, n, p.qs[m]);
+  w8_finish4<O>(p, a, w8_channels(p, n), m, n, p.qs[m]);
 }
 
 template <int TM, bool SPLIT, typename O>
@@ -717,11 +752,228 @@ static int launch_few_float(const PhW8Params& p, int x_type, const FloatRows& f,
   }
 }
 
-static int launch_product(const PhW8Params& p, const Choice& c, int out_type, hipStream_t st) {
+// Long rows of a large output go past the caches: 120704 x 512 bf16 of K = 384 69 -> 55 us, 16384 x 4096 of K = 4096 263 ->
+// 247 us.  Rows that end inside a line lose by it (N = 52: 17.5 -> 18.7 us).
+static int launch_product(PhW8Params p, const Choice& c, int out_type, hipStream_t st) {
+  const int64_t row = (int64_t)p.N * (out_type == PH_F32 ? 4 : 2);
+  p.stream = row >= 512 && row * p.M >= (4 << 20);
   switch (out_type) {
     case PH_F32: return launch_product_t<float>(p, c, st);
     case PH_F16: return launch_product_t<_Float16>(p, c, st);
     default: return launch_product_t<bf16>(p, c, st);
+  }
+}
+
+// ---- two layers --------------------------------------------------------------------------------------------------------
+//
+// x [.., 8 <= K <= 512] -> H <= 512 -> N <= 64 in one kernel: the inner rows never leave the CU.  A block owns 16 TF tokens at a
+// time and all H inner channels, 64 to a wave: their sums fill its registers, so the maximum of an inner row, which the
+// second quantisation needs, is known before anything is rounded.  Per tile: the rows are quantised into LDS; first product
+// (weights straight from cache, each fragment read by one wave and used for TF products); inner values and their maxima;
+// inner rows in 8 bits into the same LDS; second product, its weights in LDS for good.  Two blocks share a CU, so that one's
+// rounding (12 vector operations per inner value) runs under the other's products.
+#define PAIR_MAX 512   // widest input and widest inner row
+struct PhW8Pair {
+  const void* x;
+  PhRowMap xr;
+  unsigned M;
+  int K, H, N, nkb1, nnb1, nkb2, nnb2, act1, act2;
+  const int8_t *w1, *w2;
+  const float *ws1, *bias1, *slope1, *ws2, *bias2, *slope2;
+  void* out;
+  PhRowMap outr;
+  int out_type;
+};
+
+template <int TF, int ACT, typename T>
+__global__ __launch_bounds__(512, 4) void w8_pair_kernel(const PhW8Pair p) {
+  constexpr int BT = 16 * TF, RP = BT / 32, CH = 4;   // 16 lanes a row, 32 rows at a time, 4 chunks of 128 values
+  constexpr int PITCH = PAIR_MAX + 16;                // of a row in LDS: 16 rows' units lie in different banks
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  char* const q = lds;                                // the rows in 8 bits, then the inner rows
+  float* const s1 = (float*)(q + BT * PITCH);
+  float* const s2 = s1 + BT;
+  float* const red = s2 + BT;                         // [8][BT]
+  float* const par = red + 8 * BT;                    // scale, bias, slope of the inner channels [3][PAIR_MAX]
+  char* const w2 = (char*)(par + 3 * PAIR_MAX);
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int fr = lane & 15, fq = lane >> 4;
+  const unsigned m0 = blockIdx.x * BT;
+  const int K = p.K;
+  {   // rows -> q, s1
+    Eight<T> raw[RP][CH];
+#pragma unroll
+    for (int r = 0; r < RP; r++) {
+      const T* row = (const T*)p.x + ph_row_off(p.xr, min(m0 + r * 32 + (tid >> 4), p.M - 1));
+#pragma unroll
+      for (int c = 0; c < CH; c++)
+        if (c * 128 < K) raw[r][c].load_long(row, c * 128 + (tid & 15) * 8, K);
+    }
+    for (int n = tid; n < PAIR_MAX; n += 512) {   // (channels that do not exist: zeros)
+      const bool is = n < p.nnb1 * 16;
+      par[n] = is ? p.ws1[n] : 0.f;
+      par[PAIR_MAX + n] = is && p.bias1 ? p.bias1[n] : 0.f;
+      par[2 * PAIR_MAX + n] = is && p.slope1 ? p.slope1[n] : 0.f;
+    }
+    for (int f = wave; f < p.nnb2 * p.nkb2; f += 8)
+      __builtin_amdgcn_global_load_lds((glb_void*)(p.w2 + f * 1024 + lane * 16), (lds_void*)(w2 + f * 1024), 16, 0, 0);
+#pragma unroll
+    for (int r = 0; r < RP; r++) {
+      float am = 0.f;
+#pragma unroll
+      for (int c = 0; c < CH; c++)
+        if (c * 128 < K) am = raw[r][c].max_with(am);
+      const RowScale sc = row_scale(max_group<16>(am));
+      const int t = r * 32 + (tid >> 4);
+      if ((tid & 15) == 0) s1[t] = scale_out(sc);
+#pragma unroll
+      for (int c = 0; c < CH; c++) {
+        const int k = c * 128 + (tid & 15) * 8;
+        if (k < K) *(uint64_t*)(q + t * PITCH + k) = raw[r][c].quantize(sc) >> Eight<T>::shift(k, K);
+      }
+    }
+  }
+  const int8_t* wp[4];
+#pragma unroll
+  for (int j = 0; j < 4; j++) wp[j] = p.w1 + (int64_t)min(wave * 4 + j, p.nnb1 - 1) * p.nkb1 * 1024 + lane * 16;
+  i32x4 wa[4], wb[4];
+#pragma unroll
+  for (int j = 0; j < 4; j++) wa[j] = *(const i32x4*)wp[j];
+  __syncthreads();
+  i32x4 acc[4][TF];
+#pragma unroll
+  for (int j = 0; j < 4; j++)
+#pragma unroll
+    for (int i = 0; i < TF; i++) acc[j][i] = i32x4{0, 0, 0, 0};
+  const char* const xq = q + fr * PITCH + fq * 16;
+  for (int kb = 0; kb < p.nkb1; kb += 2) {
+#pragma unroll
+    for (int j = 0; j < 4; j++) wb[j] = *(const i32x4*)(wp[j] + (kb + 1) * 1024);
+#pragma unroll
+    for (int i = 0; i < TF; i++) {
+      const i32x4 xf = *(const i32x4*)(xq + i * 16 * PITCH + kb * 64);
+#pragma unroll
+      for (int j = 0; j < 4; j++) acc[j][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wa[j], xf, acc[j][i], 0, 0, 0);
+    }
+    const int nx = min(kb + 2, p.nkb1 - 1);
+#pragma unroll
+    for (int j = 0; j < 4; j++) wa[j] = *(const i32x4*)(wp[j] + nx * 1024);
+#pragma unroll
+    for (int i = 0; i < TF; i++) {
+      const i32x4 xf = *(const i32x4*)(xq + i * 16 * PITCH + kb * 64 + 64);
+#pragma unroll
+      for (int j = 0; j < 4; j++) acc[j][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wb[j], xf, acc[j][i], 0, 0, 0);
+    }
+  }
+  // inner values, in place of their sums, and each row's maximum
+  float am[TF], sc[TF];
+#pragma unroll
+  for (int i = 0; i < TF; i++) am[i] = 0.f, sc[i] = s1[i * 16 + fr];
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    const int n = (wave * 4 + j) * 16 + fq * 4;
+    Channels c;
+    c.ws = *(const f32x4*)(par + n);
+    c.bias = *(const f32x4*)(par + PAIR_MAX + n);
+    c.slope = *(const f32x4*)(par + 2 * PAIR_MAX + n);
+#pragma unroll
+    for (int i = 0; i < TF; i++) {
+      const f32x4 v = w8_values<ACT>(acc[j][i], c, sc[i]);
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        acc[j][i][e] = (int)__float_as_uint(v[e]);
+        am[i] = max_abs(am[i], v[e]);
+      }
+      __builtin_amdgcn_sched_barrier(0);   // (all at once they would not fit the registers)
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < TF; i++) {
+    am[i] = max_32(max_16(am[i]));
+    if (fq == 0) red[wave * BT + i * 16 + fr] = am[i];
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the second layer's weights are in LDS
+  __syncthreads();   // the first product is done everywhere: q is free
+#pragma unroll
+  for (int i = 0; i < TF; i++) {
+    float a = 0.f;
+#pragma unroll
+    for (int w = 0; w < 8; w++) a = max_abs(a, red[w * BT + i * 16 + fr]);
+    const RowScale r = row_scale(a);
+    if (wave == 0 && fq == 0) s2[i * 16 + fr] = scale_out(r);
+    float v[16];
+    unsigned o[4];
+#pragma unroll
+    for (int e = 0; e < 16; e++) v[e] = __uint_as_float((unsigned)acc[e >> 2][i][e & 3]);
+    quantize_n(v, r, o);
+#pragma unroll
+    for (int j = 0; j < 4; j++) *(unsigned*)(q + (i * 16 + fr) * PITCH + (wave * 4 + j) * 16 + fq * 4) = o[j];
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  __syncthreads();
+  // second product: a wave has one fragment of channels and every dt-th fragment of tokens
+  const int div = p.nnb2 > 2 ? 4 : p.nnb2, nb2 = wave % div, t0 = wave / div, dt = 8 / div;
+  constexpr int U = TF / 2;
+  i32x4 z[U];
+#pragma unroll
+  for (int u = 0; u < U; u++) z[u] = i32x4{0, 0, 0, 0};
+  const int n = nb2 * 16 + fq * 4;
+  PhW8Params o;
+  o.ws = p.ws2, o.bias = p.bias2, o.slope = p.slope2, o.act = p.act2, o.N = p.N, o.out = p.out, o.outr = p.outr;
+  const Channels c2 = w8_channels(o, min(n, p.nnb2 * 16 - 4));
+  const char* const wq = w2 + min(nb2, p.nnb2 - 1) * p.nkb2 * 1024 + lane * 16;
+  for (int kb = 0; kb < p.nkb2; kb++) {
+    const i32x4 w = *(const i32x4*)(wq + kb * 1024);
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      const int i = t0 + u * dt;
+      if (i < TF) z[u] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w, *(const i32x4*)(xq + i * 16 * PITCH + kb * 64), z[u], 0, 0, 0);
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < U; u++) {
+    const int i = t0 + u * dt;
+    const unsigned m = m0 + i * 16 + fr;
+    if (i < TF && m < p.M && n < p.N && nb2 < p.nnb2) {
+      const float s = s2[i * 16 + fr];
+      if (p.out_type == PH_F32) w8_finish4<float>(o, z[u], c2, m, n, s);
+      else if (p.out_type == PH_F16) w8_finish4<_Float16>(o, z[u], c2, m, n, s);
+      else w8_finish4<bf16>(o, z[u], c2, m, n, s);
+    }
+  }
+}
+
+static bool pair_fits(int K, int H, int N) { return K >= 8 && K <= PAIR_MAX && H <= PAIR_MAX && N <= 64; }
+
+template <int TF, int ACT, typename T>
+static int launch_pair_f(const PhW8Pair& p, hipStream_t st) {
+  constexpr int BT = 16 * TF;
+  const int lds = BT * (PAIR_MAX + 16) + 10 * BT * 4 + 12 * PAIR_MAX + p.nnb2 * p.nkb2 * 1024;   // <= 74 KB: two blocks a CU
+  static int granted[PH_MAX_DEVICES];
+  if (lds > 64 * 1024 && ph_ensure_lds((const void*)w8_pair_kernel<TF, ACT, T>, lds, granted)) return -1;
+  hipLaunchKernelGGL((w8_pair_kernel<TF, ACT, T>), dim3((p.M - 1) / BT + 1), dim3(512), lds, st, p);
+  PH_CHECK(hipGetLastError());
+  return 0;
+}
+template <int ACT, typename T>
+static int launch_pair_t(const PhW8Pair& p, hipStream_t st) {
+  // 32 tokens a block fill the chip earlier (15088 tokens of 384 -> 512 -> 26: 13.6 against 14.5 us), 64 read the first
+  // weights half as often (30176: 22.4 against 24.0, 120704: 80 against 91)
+  return p.M <= 20000 ? launch_pair_f<2, ACT, T>(p, st) : launch_pair_f<4, ACT, T>(p, st);
+}
+template <int ACT>
+static int launch_pair_a(const PhW8Pair& p, int x_type, hipStream_t st) {
+  switch (x_type) {
+    case PH_F32: return launch_pair_t<ACT, float>(p, st);
+    case PH_F16: return launch_pair_t<ACT, _Float16>(p, st);
+    default: return launch_pair_t<ACT, bf16>(p, st);
+  }
+}
+static int launch_pair(const PhW8Pair& p, int x_type, hipStream_t st) {
+  switch (p.act1) {
+    case PH_ACT_RELU: return launch_pair_a<PH_ACT_RELU>(p, x_type, st);
+    case PH_ACT_PRELU: return launch_pair_a<PH_ACT_PRELU>(p, x_type, st);
+    default: return launch_pair_a<PH_ACT_NONE>(p, x_type, st);
   }
 }
 
@@ -829,6 +1081,7 @@ PhW8Params product_params(const int8_t* q, const PhRowMap& qr, const float* qs, 
   PhW8Params p;
   p.q = q, p.qr = qr, p.qs = qs, p.w = l.packed, p.ws = l.scale, p.bias = l.bias, p.slope = l.slope, p.act = l.act;
   p.parts = parts;
+  p.stream = 0;
   p.M = M, p.N = l.n, p.K = l.k, p.nkb = nkb_of(l.k), p.nnb = (l.n + 15) / 16, p.out = out, p.outr = outr;
   return p;
 }
@@ -932,7 +1185,7 @@ int64_t ph_w8_workspace(int op, int64_t m, int k, int h, int n) {
         ph_set_error("ph_w8_workspace: a feed-forward's inner width is 1 or more");
         return -1;
       }
-      return PairSpace(nullptr, m, k, h, n).used();
+      return pair_fits(k, h, n) ? 0 : PairSpace(nullptr, m, k, h, n).used();
     default:
       ph_set_error("ph_w8_workspace: unknown operator %d", op);
       return -1;
@@ -1013,12 +1266,19 @@ int ph_w8_feed_forward(int device, void* stream, const void* x, int x_type, cons
   if (M == 0) return 0;
   if (!some(who, x, out) || !some(who, out, out_stride)) return -1;
   const int K = layer1->k, H = layer1->n;
-  const PairSpace w(ws, M, K, H, layer2->n);
-  if (!ws_ok(who, ws, ws_bytes, w.used())) return -3;
   ph_rows orow = *rows;
   for (int d = 0; d < 3; d++) orow.stride[d] = out_stride[d];
-  W8_DEVICE(device);
   hipStream_t st = (hipStream_t)stream;
+  if (pair_fits(K, H, layer2->n)) {
+    W8_DEVICE(device);
+    const ph_w8_layer &a = *layer1, &b = *layer2;
+    const PhW8Pair p = {x, row_map(*rows), (unsigned)M, K, H, b.n, nkb_of(K), (H + 15) / 16, nkb_of(H), (b.n + 15) / 16, a.act, b.act,
+                        a.packed, b.packed, a.scale, a.bias, a.slope, b.scale, b.bias, b.slope, out, row_map(orow), out_type};
+    return launch_pair(p, x_type, st);
+  }
+  const PairSpace w(ws, M, K, H, layer2->n);
+  if (!ws_ok(who, ws, ws_bytes, w.used())) return -3;
+  W8_DEVICE(device);
   const int64_t pitch = q_pitch_of(K), hpitch = up(H, 4), pitch2 = q_pitch_of(H);
   if (quantize(x, x_type, row_map(*rows), (unsigned)M, K, w.a.q, pitch, w.a.s, st)) return -1;
   if (launch_product(product_params(w.a.q, even_rows(pitch), w.a.s, (unsigned)M, *layer1, w.h, even_rows(hpitch), w.a.parts),

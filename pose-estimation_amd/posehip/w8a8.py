@@ -286,8 +286,8 @@ def feed_forward(x, layer1, layer2, out=None, dtype=None):
     y, rows, ostride, m = _output(x, layer2.n, out, dtype, x.dtype)
     if m:
         need = _workspace(_ffi.PH_W8_FEED_FORWARD, m, layer1.k, layer1.n, layer2.n)
-        ws = torch.empty(need, dtype=torch.int8, device=x.device)
+        ws = torch.empty(need, dtype=torch.int8, device=x.device) if need else None
         _ffi.check(_ffi.lib().ph_w8_feed_forward(x.device.index, _stream(x.device), x.data_ptr(), _TYPES[x.dtype], rows,
                                                  layer1.desc, layer2.desc, y.data_ptr(), _TYPES[y.dtype], ostride,
-                                                 ws.data_ptr(), need), "ph_w8_feed_forward")
+                                                 ws.data_ptr() if need else None, need), "ph_w8_feed_forward")
     return y

@@ -84,7 +84,7 @@ def test_c_refusals():
                                       st, k.get("ws", 4096), k.get("nws", 1 << 20))
     assert li(x=None) == -1 and li(t=5) == -1 and li(ot=5) == -1 and li(ws=None) == -3 and li(nws=100) == -3
     ff = lambda a, b, **k: lib.ph_w8_feed_forward(0, None, 4096, 0, rows(), a, b, 4096, 0, st, 4096, k.get("nws", 1 << 20))   # noqa: E731
-    assert ff(layer(n=16), layer(k=64)) == -1 and ff(layer(n=64), layer(k=64), nws=64) == -3
+    assert ff(layer(n=16), layer(k=64)) == -1 and ff(layer(n=640), layer(k=640), nws=64) == -3
     assert ff(layer(n=64), layer(k=64, n=0)) == -1
 
 
