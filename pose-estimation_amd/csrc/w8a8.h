@@ -36,3 +36,37 @@ struct PhW8Params {
   PhRowMap outr;
   int* parts;            // split along K: sums [part][M][N16]
 };
+
+// How a product is done: which kernel, and in how many parts along K.
+struct PhW8Choice {
+  int kernel, parts;
+};
+PhW8Choice ph_w8_choose(int64_t M, int N, int nkb);
+int64_t ph_w8_parts_bytes(const PhW8Choice& c, int64_t M, int N);
+int ph_launch_w8_product(const PhW8Params& p, const PhW8Choice& c, int out_type, hipStream_t st);
+
+// Float rows that a product's blocks quantise themselves (p.q, p.qr and p.qs are not used).
+struct FloatRows {
+  const void* x;
+  PhRowMap r;
+};
+bool ph_w8_few_float(int64_t M, int K);
+int ph_launch_w8_few_float(const PhW8Params& p, const FloatRows& f, int x_type, int out_type, hipStream_t st);
+
+#define PAIR_MAX 512   // widest rows of the kernels that quantise them themselves, and widest inner rows
+bool ph_w8_rows_fit(int64_t M, int K, int N);
+int ph_launch_w8_rows(const PhW8Params& p, const FloatRows& f, int x_type, int out_type, hipStream_t st);
+
+struct PhW8Pair {
+  const void* x;
+  PhRowMap xr;
+  unsigned M;
+  int K, H, N, nkb1, nnb1, nkb2, nnb2, act1, act2;
+  const int8_t *w1, *w2;
+  const float *ws1, *bias1, *slope1, *ws2, *bias2, *slope2;
+  void* out;
+  PhRowMap outr;
+  int out_type;
+};
+bool ph_w8_pair_fits(int K, int H, int N);
+int ph_launch_w8_pair(const PhW8Pair& p, int x_type, hipStream_t st);

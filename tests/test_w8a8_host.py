@@ -80,7 +80,7 @@ def test_c_refusals():
     assert m(out=None) == -1 and m(st=None) == -1 and m(rows=None) == -1
     assert m(q=4097) == -3 and m(rows=rows(stride=(0, 0, 65))) == -3 and m(q=4097, ws=4096 + 16, nws=1 << 20) == -3
     assert b"workspace" in lib.ph_last_error()
-    li = lambda **k: lib.ph_w8_linear(0, None, k.get("x", 4096), k.get("t", 0), k.get("rows", rows((1, 1, 100))), layer(), 4096, k.get("ot", 0),   # noqa: E731
+    li = lambda **k: lib.ph_w8_linear(0, None, k.get("x", 4096), k.get("t", 0), k.get("rows", rows((1, 1, 100))), layer(k=4000), 4096, k.get("ot", 0),   # noqa: E731
                                       st, k.get("ws", 4096), k.get("nws", 1 << 20))
     assert li(x=None) == -1 and li(t=5) == -1 and li(ot=5) == -1 and li(ws=None) == -3 and li(nws=100) == -3
     ff = lambda a, b, **k: lib.ph_w8_feed_forward(0, None, 4096, 0, rows(), a, b, 4096, 0, st, 4096, k.get("nws", 1 << 20))   # noqa: E731
