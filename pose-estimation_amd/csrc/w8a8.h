@@ -21,7 +21,7 @@ __host__ __device__ static inline int64_t ph_row_off(const PhRowMap& r, unsigned
 }
 
 struct PhW8Params {
-  const int8_t* q;       // 8-bit rows, K contiguous values each (rows 16-byte aligned)
+  const int8_t* q;       // 8-bit rows, K contiguous values each (rows 16-byte aligned, unless loose)
   PhRowMap qr;
   const float* qs;       // scale of each row [M]
   const int8_t* w;       // packed weight fragments [N16/16][K128/64][1024]
@@ -30,6 +30,7 @@ struct PhW8Params {
   const float* slope;    // [N16] or NULL
   int act;
   int stream;            // store past the caches
+  int loose;             // rows start anywhere (ph_w8_loose() says whether the product takes that)
   unsigned M;
   int N, K, nkb, nnb;    // nkb = K128 / 64 fragments along K (even), nnb = N16 / 16 along N
   void* out;
@@ -42,6 +43,7 @@ struct PhW8Choice {
   int kernel, parts;
 };
 PhW8Choice ph_w8_choose(int64_t M, int N, int nkb);
+bool ph_w8_loose(int64_t M, int K, int N);
 int64_t ph_w8_parts_bytes(const PhW8Choice& c, int64_t M, int N);
 int ph_launch_w8_product(const PhW8Params& p, const PhW8Choice& c, int out_type, hipStream_t st);
 

@@ -106,19 +106,30 @@ __global__ void pack_weight_kernel(const int8_t* __restrict__ w, int64_t row_str
   *(u32x4*)(out + t * 16) = p.v;
 }
 
-// rows of any alignment -> rows of `pitch` bytes, 16-byte aligned
+// rows of any alignment -> rows of `pitch` bytes, 16-byte aligned; a thread moves 4 pieces of 16 bytes of a row
 __global__ void repitch_kernel(const int8_t* __restrict__ q, PhRowMap qr, unsigned M, int K, int8_t* __restrict__ out,
                                int64_t pitch) {
-  const int64_t ppr = pitch >> 4;
+  typedef u32x4 u16b __attribute__((aligned(1)));
+  const int per = (int)((pitch + 63) >> 6);   // threads of a row
   const int64_t t = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  if (t >= (int64_t)M * ppr) return;
-  const unsigned m = (unsigned)(t / ppr);
-  const int k = (int)(t - m * ppr) * 16;
+  const unsigned m = (unsigned)(t / per);
+  if (m >= M) return;
+  const int p0 = (int)(t - (int64_t)m * per);
   const int8_t* row = q + ph_row_off(qr, m);
-  union { int8_t b[16]; u32x4 v; } p;
+  int8_t* const to = out + (int64_t)m * pitch;
+  u32x4 v[4];
 #pragma unroll
-  for (int i = 0; i < 16; i++) p.b[i] = k + i < K ? row[k + i] : (int8_t)0;
-  *(u32x4*)(out + (int64_t)m * pitch + k) = p.v;
+  for (int u = 0; u < 4; u++) {
+    const int k = (p0 + u * per) * 16;
+    if (k + 16 <= K) v[u] = *(const u16b*)(row + k);
+  }
+#pragma unroll
+  for (int u = 0; u < 4; u++) {
+    const int k = (p0 + u * per) * 16;
+    if (k + 16 <= K) *(u32x4*)(to + k) = v[u];
+    else
+      for (int i = k; i < K; i++) to[i] = row[i];
+  }
 }
 
 // ---- entry points --------------------------------------------------------------------------------------------------------
@@ -225,6 +236,7 @@ PhW8Params product_params(const int8_t* q, const PhRowMap& qr, const float* qs, 
   PhW8Params p;
   p.q = q, p.qr = qr, p.qs = qs, p.w = l.packed, p.ws = l.scale, p.bias = l.bias, p.slope = l.slope, p.act = l.act;
   p.parts = parts;
+  p.loose = 0;
   // Long rows of a large output go past the caches: 120704 x 512 bf16 of K = 384 69 -> 55 us, 16384 x 4096 of K = 4096
   // 263 -> 247 us.  Rows that end inside a line lose by it (N = 52: 17.5 -> 18.7 us).
   const int64_t row = (int64_t)l.n * (out_type == PH_F32 ? 4 : 2);
@@ -264,16 +276,29 @@ struct RowsSpace {
   }
   int64_t used() const { return w.used; }
 };
-// Of two layers: the inner rows in f32, and the larger of the two products' spaces, one after the other in one place.
-struct PairSpace {
-  float* h;
-  RowsSpace a, b;
-  int64_t hbytes;
-  PairSpace(void* ws, int64_t M, int K, int H, int N)
-      : h((float*)ws), a((char*)ws + up(M * up(H, 4) * 4, 256), M, K, H, true, true),
-        b((char*)ws + up(M * up(H, 4) * 4, 256), M, H, N, true, true), hbytes(up(M * up(H, 4) * 4, 256)) {}
-  int64_t used() const { return hbytes + (a.used() > b.used() ? a.used() : b.used()); }
-};
+// rows of a layer that quantises them itself need no space
+bool itself(int64_t M, int K, int N) { return ph_w8_few_float(M, K) || ph_w8_rows_fit(M, K, N); }
+int64_t linear_space(int64_t M, int K, int N) { return itself(M, K, N) ? 0 : RowsSpace(nullptr, M, K, N, true, true).used(); }
+
+int linear(const void* x, int x_type, const PhRowMap& xr, unsigned M, const ph_w8_layer& l, void* out, int out_type,
+           const PhRowMap& outr, void* ws, hipStream_t st) {
+  if (itself(M, l.k, l.n)) {
+    const FloatRows f = {x, xr};
+    const PhW8Params p = product_params(nullptr, xr, nullptr, M, l, out, outr, nullptr, out_type);
+    return ph_w8_few_float(M, l.k) ? ph_launch_w8_few_float(p, f, x_type, out_type, st) : ph_launch_w8_rows(p, f, x_type, out_type, st);
+  }
+  const RowsSpace w(ws, M, l.k, l.n, true, true);
+  const int64_t pitch = q_pitch_of(l.k);
+  if (quantize(x, x_type, xr, M, l.k, w.q, pitch, w.s, st)) return -1;
+  return ph_launch_w8_product(product_params(w.q, even_rows(pitch), w.s, M, l, out, outr, w.parts, out_type), w.choice, out_type, st);
+}
+
+// Of two layers: the inner rows in f32, and the larger of the two layers' spaces, one after the other in one place.
+int64_t inner_bytes(int64_t M, int H) { return up(M * up(H, 4) * 4, 256); }
+int64_t pair_space(int64_t M, int K, int H, int N) {
+  const int64_t a = linear_space(M, K, H), b = linear_space(M, H, N);
+  return inner_bytes(M, H) + (a > b ? a : b);
+}
 
 }  // namespace
 
@@ -325,14 +350,14 @@ int64_t ph_w8_workspace(int op, int64_t m, int k, int h, int n) {
   if (m == 0) return 0;
   switch (op) {
     case PH_W8_MATMUL: return RowsSpace(nullptr, m, k, n, false, false).used();
-    case PH_W8_MATMUL_ANY: return RowsSpace(nullptr, m, k, n, true, false).used();
-    case PH_W8_LINEAR: return ph_w8_few_float(m, k) || ph_w8_rows_fit(m, k, n) ? 0 : RowsSpace(nullptr, m, k, n, true, true).used();
+    case PH_W8_MATMUL_ANY: return RowsSpace(nullptr, m, k, n, !ph_w8_loose(m, k, n), false).used();
+    case PH_W8_LINEAR: return linear_space(m, k, n);
     case PH_W8_FEED_FORWARD:
       if (h < 1) {
         ph_set_error("ph_w8_workspace: a feed-forward's inner width is 1 or more");
         return -1;
       }
-      return ph_w8_pair_fits(k, h, n) ? 0 : PairSpace(nullptr, m, k, h, n).used();
+      return ph_w8_pair_fits(k, h, n) ? 0 : pair_space(m, k, h, n);
     default:
       ph_set_error("ph_w8_workspace: unknown operator %d", op);
       return -1;
@@ -355,20 +380,21 @@ int ph_w8_matmul(int device, void* stream, const int8_t* q, const ph_rows* rows,
   ph_rows orow = *rows;
   for (int d = 0; d < 3; d++) orow.stride[d] = out_stride[d];
   PhRowMap qr = row_map(*rows);
-  const bool direct = aligned16(q, qr);
+  const bool even = aligned16(q, qr), direct = even || ph_w8_loose(M, layer->k, layer->n);
   const RowsSpace w(ws, M, layer->k, layer->n, !direct, false);
   if (!ws_ok(who, ws, ws_bytes, w.used())) return -3;
   W8_DEVICE(device);
   if (!direct) {
-    const int64_t pitch = q_pitch_of(layer->k), pieces = M * (pitch / 16);
-    hipLaunchKernelGGL(repitch_kernel, dim3((unsigned)((pieces + 255) / 256)), dim3(256), 0, (hipStream_t)stream, q, qr,
+    const int64_t pitch = q_pitch_of(layer->k), threads = M * ((pitch + 63) / 64);
+    hipLaunchKernelGGL(repitch_kernel, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, (hipStream_t)stream, q, qr,
                        (unsigned)M, layer->k, w.q, pitch);
     PH_CHECK(hipGetLastError());
     q = w.q;
     qr = even_rows(pitch);
   }
-  return ph_launch_w8_product(product_params(q, qr, scale, (unsigned)M, *layer, out, row_map(orow), w.parts, out_type), w.choice, out_type,
-                        (hipStream_t)stream);
+  PhW8Params p = product_params(q, qr, scale, (unsigned)M, *layer, out, row_map(orow), w.parts, out_type);
+  p.loose = direct && !even;
+  return ph_launch_w8_product(p, w.choice, out_type, (hipStream_t)stream);
 }
 
 int ph_w8_linear(int device, void* stream, const void* x, int x_type, const ph_rows* rows, const ph_w8_layer* layer, void* out,
@@ -380,21 +406,9 @@ int ph_w8_linear(int device, void* stream, const void* x, int x_type, const ph_r
   if (!some(who, x, out) || !some(who, out, out_stride)) return -1;
   ph_rows orow = *rows;
   for (int d = 0; d < 3; d++) orow.stride[d] = out_stride[d];
-  hipStream_t st = (hipStream_t)stream;
-  const PhRowMap xr = row_map(*rows), outr = row_map(orow);
-  const bool few = ph_w8_few_float(M, layer->k);
-  if (few || ph_w8_rows_fit(M, layer->k, layer->n)) {
-    W8_DEVICE(device);
-    const FloatRows f = {x, xr};
-    const PhW8Params p = product_params(nullptr, xr, nullptr, (unsigned)M, *layer, out, outr, nullptr, out_type);
-    return few ? ph_launch_w8_few_float(p, f, x_type, out_type, st) : ph_launch_w8_rows(p, f, x_type, out_type, st);
-  }
-  const int64_t pitch = q_pitch_of(layer->k);
-  const RowsSpace w(ws, M, layer->k, layer->n, true, true);
-  if (!ws_ok(who, ws, ws_bytes, w.used())) return -3;
+  if (!ws_ok(who, ws, ws_bytes, linear_space(M, layer->k, layer->n))) return -3;
   W8_DEVICE(device);
-  if (quantize(x, x_type, xr, (unsigned)M, layer->k, w.q, pitch, w.s, st)) return -1;
-  return ph_launch_w8_product(product_params(w.q, even_rows(pitch), w.s, (unsigned)M, *layer, out, outr, w.parts, out_type), w.choice, out_type, st);
+  return linear(x, x_type, row_map(*rows), (unsigned)M, *layer, out, out_type, row_map(orow), ws, (hipStream_t)stream);
 }
 
 int ph_w8_feed_forward(int device, void* stream, const void* x, int x_type, const ph_rows* rows, const ph_w8_layer* layer1,
@@ -420,16 +434,13 @@ int ph_w8_feed_forward(int device, void* stream, const void* x, int x_type, cons
                         a.packed, b.packed, a.scale, a.bias, a.slope, b.scale, b.bias, b.slope, out, row_map(orow), out_type};
     return ph_launch_w8_pair(p, x_type, st);
   }
-  const PairSpace w(ws, M, K, H, layer2->n);
-  if (!ws_ok(who, ws, ws_bytes, w.used())) return -3;
+  if (!ws_ok(who, ws, ws_bytes, pair_space(M, K, H, layer2->n))) return -3;
   W8_DEVICE(device);
-  const int64_t pitch = q_pitch_of(K), hpitch = up(H, 4), pitch2 = q_pitch_of(H);
-  if (quantize(x, x_type, row_map(*rows), (unsigned)M, K, w.a.q, pitch, w.a.s, st)) return -1;
-  if (ph_launch_w8_product(product_params(w.a.q, even_rows(pitch), w.a.s, (unsigned)M, *layer1, w.h, even_rows(hpitch), w.a.parts, PH_F32),
-                     w.a.choice, PH_F32, st)) return -1;
-  if (quantize(w.h, PH_F32, even_rows(hpitch), (unsigned)M, H, w.b.q, pitch2, w.b.s, st)) return -1;
-  return ph_launch_w8_product(product_params(w.b.q, even_rows(pitch2), w.b.s, (unsigned)M, *layer2, out, row_map(orow), w.b.parts, out_type),
-                        w.b.choice, out_type, st);
+  float* const h = (float*)ws;
+  void* const more = (char*)ws + inner_bytes(M, H);
+  const PhRowMap inner = even_rows(up(H, 4));
+  if (linear(x, x_type, row_map(*rows), (unsigned)M, *layer1, h, PH_F32, inner, more, st)) return -1;
+  return linear(h, PH_F32, inner, (unsigned)M, *layer2, out, out_type, row_map(orow), more, st);
 }
 
 }  // extern "C"

@@ -218,6 +218,24 @@ __device__ __forceinline__ void quantize_block(const FloatRows& f, unsigned M, i
   __syncthreads();
 }
 
+// 16 bytes of a row of K >= 16 that starts anywhere, nothing read behind its end: where fewer are left, its last 16 and a
+// shift (the same in every lane that has one; what moves in meets zero weights)
+__device__ __forceinline__ i32x4 load_loose(const int8_t* row, int k, int K) {
+  typedef i32x4 any __attribute__((aligned(1)));
+  const int over = k + 16 - K;
+  i32x4 v = *(const any*)(row + (over > 0 ? K - 16 : k));
+  const int b = 16 - (K & 15);   // of the piece that the row's end cuts
+  if (over > 0) {
+    if (b & 8) v = i32x4{v[2], v[3], 0, 0};
+    if (b & 4) v = i32x4{v[1], v[2], v[3], 0};
+    const int bs = b & 3;
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+      v[i] = (int)__builtin_amdgcn_alignbyte(i < 3 ? (unsigned)v[i + 1] : 0u, (unsigned)v[i], bs);
+  }
+  return v;
+}
+
 template <int TM, int W, bool SPLIT, typename T, typename O>
 __global__ __launch_bounds__(64 * W) void w8_few_kernel(const PhW8Params p, const FloatRows f) {
   constexpr bool FLOAT = !__is_same(T, int8_t);
@@ -261,6 +279,7 @@ __global__ __launch_bounds__(64 * W) void w8_few_kernel(const PhW8Params p, cons
 #pragma unroll
       for (int i = 0; i < TM; i++) {
         if constexpr (FLOAT) xf[d][i] = *(const i32x4*)(s_q + xq[i] + k);
+        else if (p.loose) xf[d][i] = load_loose(xp[i], k, p.K);
         else xf[d][i] = *(const i32x4*)(xp[i] + k);
       }
       w[d] = wf[d];
@@ -359,6 +378,10 @@ PhW8Choice ph_w8_choose(int64_t M, int N, int nkb) {
     }
   }
   return best;
+}
+
+bool ph_w8_loose(int64_t M, int K, int N) {
+  return K >= 16 && M <= 64 && ph_w8_choose(M, N, (int)((K + 127) / 128 * 2)).kernel == K_FEW;
 }
 
 int64_t ph_w8_parts_bytes(const PhW8Choice& c, int64_t M, int N) {
