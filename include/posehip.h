@@ -31,6 +31,10 @@ typedef struct ph_ctx ph_ctx;
 #define PH_MAX_DST 8
 #define PH_OP_CONV 0
 #define PH_OP_POOL 1
+/* A 1x1 conv in 8-bit integers, a scale per pixel and per output channel (see "8-bit products" below); kh = kw = 1, no
+ * pooling.  Such ops come in pairs: the first one's output (<= 512 channels of <= 512) is read by the second only (<= 64
+ * channels); the values between them stay f32 until they are quantised. */
+#define PH_OP_CONV_W8A8 2
 #define PH_ACT_NONE 0
 #define PH_ACT_RELU 1
 #define PH_ACT_PRELU 2
@@ -47,7 +51,7 @@ typedef struct {
 /* One fused operation of the execution plan (built by posehip/graph.py from the
  * Caffe prototxt the reference hands to readNetFromCaffe / OpenPose). */
 typedef struct {
-  int type;                 /* PH_OP_CONV | PH_OP_POOL */
+  int type;                 /* PH_OP_CONV | PH_OP_POOL | PH_OP_CONV_W8A8 */
   int in_buf, in_coff;      /* input buffer id, first channel read */
   int cin_read;             /* channels read (multiple of 8) */
   int kh, kw;               /* odd kernel, stride 1, pad = (k-1)/2 ("same") */

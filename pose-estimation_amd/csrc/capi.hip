@@ -14,6 +14,7 @@
 #include "common.h"
 #include "decode_v1.h"
 #include "decode_v2.h"
+#include "w8a8.h"
 
 int ph_launch_conv(const PhConvParams& p, int nrep, int variant, hipStream_t stream);
 bool ph_conv_halo_plan(PhConvParams& p, int kh, bool has_f32);
@@ -99,6 +100,11 @@ struct Op {
   // whenever ph_pair_enabled(); both keep their own parameters for the separate launches
   bool pair_head = false, pair = false;
   PhPairParams pp;
+  // 8-bit pair (PH_OP_CONV_W8A8): packed weights and {scale, bias, slope} of each; the second runs both
+  int8_t* w8 = nullptr;
+  float* w8_par = nullptr;
+  bool w8_head = false, w8_pair = false;
+  PhW8Pair wp;
 };
 
 struct ph_ctx {
@@ -206,6 +212,8 @@ static void free_net(ph_ctx* c) {
     if (o.bias) (void)hipFree(o.bias);
     if (o.slope) (void)hipFree(o.slope);
     if (o.tile_ctr) (void)hipFree(o.tile_ctr);
+    if (o.w8) (void)hipFree(o.w8);
+    if (o.w8_par) (void)hipFree(o.w8_par);
   }
   c->bufs.clear();
   c->ops.clear();
@@ -295,6 +303,46 @@ int ph_net_build(ph_ctx* c, int batch, const ph_buf_desc* bufs, int n_bufs, cons
   return rc;
 }
 
+// The weights of an 8-bit layer, quantised per output channel as ph_w8_quantize_rows does (two f32 numbers have no quotient
+// within 2^-53 of a border but on it, so f64 decides as the exact quotient does) and packed as ph_w8_pack does.
+static int w8_weights(Op& o, const ph_op_desc& d, int op, const std::vector<float>& bias, const std::vector<float>& slope) {
+  const int n16 = (d.cout + 15) / 16 * 16, nkb = (d.cin_read + 127) / 128 * 2;
+  std::vector<int8_t> w((size_t)n16 * nkb * 64, 0);
+  std::vector<float> par((size_t)3 * n16, 0.f);
+  for (int n = 0; n < d.cout; n++) {
+    const float* src = d.weight + (size_t)n * d.cin_caffe;
+    float amax = 0.f;
+    for (int k = 0; k < d.cin_read; k++)
+      if (d.cin_map[k] >= 0) {
+        const float a = fabsf(src[d.cin_map[k]]);
+        if (!(a <= 3.402823466e38f)) {
+          ph_set_error("ph_net_build: op %d: weight %d,%d is not finite", op, n, d.cin_map[k]);
+          return -1;
+        }
+        if (a > amax) amax = a;
+      }
+    const float s = amax / 127.f > 0x1p-126f ? amax / 127.f : 0x1p-126f;
+    par[n] = s;
+    par[n16 + n] = bias[n];
+    par[2 * n16 + n] = slope[n];
+    for (int k = 0; k < d.cin_read; k++)
+      if (d.cin_map[k] >= 0)
+        w[((size_t)(n / 16) * nkb + k / 64) * 1024 + ((k % 64) / 16 * 16 + n % 16) * 16 + k % 16] =
+            (int8_t)nearbyint((double)src[d.cin_map[k]] / (double)s);
+  }
+  PH_CHECK(hipMalloc(&o.w8, w.size()));
+  PH_CHECK(hipMalloc(&o.w8_par, par.size() * sizeof(float)));
+  PH_CHECK(hipMemcpy(o.w8, w.data(), w.size(), hipMemcpyHostToDevice));
+  PH_CHECK(hipMemcpy(o.w8_par, par.data(), par.size() * sizeof(float), hipMemcpyHostToDevice));
+  return 0;
+}
+
+// rows of a [B][Hp][Wp][Cs] buffer's H x W interior pixels
+static PhRowMap pixel_rows(int H, int W, int64_t image, int64_t line, int64_t pixel) {
+  PhRowMap r = {(unsigned)H, (unsigned)W, 0, image, line, pixel};
+  return r;
+}
+
 static int net_build(ph_ctx* c, int batch, const ph_buf_desc* bufs, int n_bufs, const ph_op_desc* ops, int n_ops,
                      int out_channels, int out_h, int out_w) {
   PH_CHECK(hipSetDevice(c->device));
@@ -360,7 +408,8 @@ static int net_build(ph_ctx* c, int batch, const ph_buf_desc* bufs, int n_bufs, 
       }
       continue;
     }
-    if (d.type != PH_OP_CONV) {
+    const bool w8 = d.type == PH_OP_CONV_W8A8;
+    if (d.type != PH_OP_CONV && !w8) {
       ph_set_error("ph_net_build: op %d: unknown type %d", i, d.type);
       return -1;
     }
@@ -379,6 +428,10 @@ static int net_build(ph_ctx* c, int batch, const ph_buf_desc* bufs, int n_bufs, 
     if (d.pool && (d.kh != 3 || (d.cin_read & 31) || ((in.d.height | in.d.width) & 1) || d.f32_coff >= 0 ||
                    d.n_dst < 1)) {
       ph_set_error("ph_net_build: op %d: fused pooling needs a 3x3 conv, cin_read %% 32 == 0, even H and W", i);
+      return -1;
+    }
+    if (w8 && (d.kh != 1 || d.pool || d.cin_read > PAIR_MAX)) {
+      ph_set_error("ph_net_build: op %d: an 8-bit layer is a 1x1 conv of at most %d channels, without pooling", i, PAIR_MAX);
       return -1;
     }
     for (int k = 0; k < d.n_dst; k++) {
@@ -514,6 +567,7 @@ static int net_build(ph_ctx* c, int batch, const ph_buf_desc* bufs, int n_bufs, 
         o.variant = 0;
       }
     }
+    if (w8 && w8_weights(o, d, i, bias, slope)) return -1;
     int real_cin = 0;
     for (int cc = 0; cc < d.cin_read; cc++) {
       real_cin += d.cin_map[cc] >= 0;
@@ -606,6 +660,45 @@ static int net_build(ph_ctx* c, int batch, const ph_buf_desc* bufs, int n_bufs, 
     a.pair_head = true;
     b.pair = true;
   }
+  // 8-bit layers: pairs like these, the first's output read by the second only
+  for (int i = 0; i < n_ops; i++) {
+    Op& a = c->ops[i];
+    if (a.d.type != PH_OP_CONV_W8A8 || a.w8_pair) continue;
+    Op* b = i + 1 < n_ops ? &c->ops[i + 1] : nullptr;
+    bool ok = b && b->d.type == PH_OP_CONV_W8A8 && a.d.n_dst == 1 && a.d.f32_coff < 0 && b->d.in_buf == a.d.dst_buf[0] &&
+              b->d.in_coff == a.d.dst_coff[0] && b->cin_span <= a.d.cout && ph_w8_pair_fits(a.d.cin_read, a.d.cout, b->d.cout);
+    for (int j = 0; ok && j < n_ops; j++) ok = j == i + 1 || c->ops[j].d.in_buf != a.d.dst_buf[0];
+    if (!ok) {
+      ph_set_error("ph_net_build: op %d: 8-bit layers come in pairs (up to %d -> %d -> 64 channels), the first one's output read "
+                   "by the second only", i, PAIR_MAX, PAIR_MAX);
+      return -1;
+    }
+    const Buf& in = c->bufs[a.d.in_buf];
+    const int H = in.d.height, W = in.d.width, n1 = (a.d.cout + 15) / 16 * 16, n2 = (b->d.cout + 15) / 16 * 16;
+    PhW8Pair& p = b->wp;
+    memset(&p, 0, sizeof(p));
+    p.x = in.ptr + in.org(0, a.d.in_coff);
+    p.xr = pixel_rows(H, W, (int64_t)in.Hp() * in.Wp() * in.d.channels, (int64_t)in.Wp() * in.d.channels, in.d.channels);
+    p.K = a.d.cin_read, p.H = a.d.cout, p.N = b->d.cout;
+    p.nkb1 = (p.K + 127) / 128 * 2, p.nnb1 = n1 / 16;
+    // (the second layer's packed weights span what it reads, which may be wider than the first layer's output)
+    p.nkb2 = (b->d.cin_read + 127) / 128 * 2, p.nnb2 = n2 / 16;
+    p.act1 = a.d.act, p.act2 = b->d.act;
+    p.w1 = a.w8, p.ws1 = a.w8_par, p.bias1 = a.w8_par + n1, p.slope1 = a.w8_par + 2 * n1;
+    p.w2 = b->w8, p.ws2 = b->w8_par, p.bias2 = b->w8_par + n2, p.slope2 = b->w8_par + 2 * n2;
+    if (b->d.f32_coff >= 0) {
+      const int64_t hw = (int64_t)H * W;
+      p.out[p.n_out++] = {c->net_out + b->d.f32_coff * hw, pixel_rows(H, W, out_channels * hw, W, 1), hw, PH_F32};
+    }
+    for (int k = 0; k < b->d.n_dst; k++) {
+      const Buf& ob = c->bufs[b->d.dst_buf[k]];
+      p.out[p.n_out++] = {ob.ptr + ob.org(0, b->d.dst_coff[k]),
+                          pixel_rows(H, W, (int64_t)ob.Hp() * ob.Wp() * ob.d.channels, (int64_t)ob.Wp() * ob.d.channels, ob.d.channels), 1, PH_BF16};
+    }
+    a.w8_head = true;
+    b->w8_pair = true;
+    i++;
+  }
   c->op_ev.resize(n_ops + 1);
   for (auto& e : c->op_ev) PH_CHECK(hipEventCreate(&e));
   c->cur_out = c->net_out;
@@ -652,7 +745,12 @@ static int run_ops(ph_ctx* c, int B, bool timed) {
     Op& o = c->ops[i];
     if (timed) PH_CHECK(hipEventRecord(c->op_ev[i], c->stream));
     const Buf& in = c->bufs[o.d.in_buf];
-    if (o.skip || (pairs && o.pair_head)) continue;
+    if (o.skip || o.w8_head || (pairs && o.pair_head)) continue;
+    if (o.w8_pair) {
+      o.wp.M = (unsigned)(B * in.d.height * in.d.width);
+      if (ph_launch_w8_pair(o.wp, PH_BF16, c->stream)) return -1;
+      continue;
+    }
     if (pairs && o.pair) {
       o.pp.a.B = B;
       o.pp.a.M = B * o.pp.a.H * o.pp.a.W;
@@ -712,7 +810,8 @@ int ph_op_kernel(ph_ctx* c, int op, char* name, int cap) {
     return -1;
   }
   const Op& o = c->ops[op];
-  if (o.skip || (o.pair_head && ph_pair_enabled())) snprintf(name, cap, "(fused into the next op)");
+  if (o.skip || o.w8_head || (o.pair_head && ph_pair_enabled())) snprintf(name, cap, "(fused into the next op)");
+  else if (o.w8_pair) snprintf(name, cap, "w8_pair_kernel<%d, %d, __bf16>", o.wp.M <= 20000 ? 2 : 4, o.wp.act1);
   else if (o.pair && ph_pair_enabled()) snprintf(name, cap, "conv1x1_pair_kernel(PhPairParams)");
   else if (o.d.type == PH_OP_POOL) snprintf(name, cap, "maxpool2x2_kernel");
   else if (o.cp.stem && ph_stem512_applies(o.cp)) snprintf(name, cap, "conv_stem512_kernel(PhConvParams, int, int, int)");

@@ -59,6 +59,12 @@ int ph_launch_w8_few_float(const PhW8Params& p, const FloatRows& f, int x_type, 
 bool ph_w8_rows_fit(int64_t M, int K, int N);
 int ph_launch_w8_rows(const PhW8Params& p, const FloatRows& f, int x_type, int out_type, hipStream_t st);
 
+struct PhW8Out {
+  void* p;
+  PhRowMap r;
+  int64_t step;          // elements from a channel to the next (1, or a plane of f32 maps)
+  int type;
+};
 struct PhW8Pair {
   const void* x;
   PhRowMap xr;
@@ -66,9 +72,8 @@ struct PhW8Pair {
   int K, H, N, nkb1, nnb1, nkb2, nnb2, act1, act2;
   const int8_t *w1, *w2;
   const float *ws1, *bias1, *slope1, *ws2, *bias2, *slope2;
-  void* out;
-  PhRowMap outr;
-  int out_type;
+  int n_out;             // the result goes to each of these
+  PhW8Out out[PH_MAX_DST + 1];
 };
 bool ph_w8_pair_fits(int K, int H, int N);
 int ph_launch_w8_pair(const PhW8Pair& p, int x_type, hipStream_t st);

@@ -430,8 +430,9 @@ int ph_w8_feed_forward(int device, void* stream, const void* x, int x_type, cons
   if (ph_w8_pair_fits(K, H, layer2->n)) {
     W8_DEVICE(device);
     const ph_w8_layer &a = *layer1, &b = *layer2;
-    const PhW8Pair p = {x, row_map(*rows), (unsigned)M, K, H, b.n, nkb_of(K), (H + 15) / 16, nkb_of(H), (b.n + 15) / 16, a.act, b.act,
-                        a.packed, b.packed, a.scale, a.bias, a.slope, b.scale, b.bias, b.slope, out, row_map(orow), out_type};
+    PhW8Pair p = {x, row_map(*rows), (unsigned)M, K, H, b.n, nkb_of(K), (H + 15) / 16, nkb_of(H), (b.n + 15) / 16, a.act, b.act,
+                  a.packed, b.packed, a.scale, a.bias, a.slope, b.scale, b.bias, b.slope, 1, {}};
+    p.out[0] = {out, row_map(orow), 1, out_type};
     return ph_launch_w8_pair(p, x_type, st);
   }
   if (!ws_ok(who, ws, ws_bytes, pair_space(M, K, H, layer2->n))) return -3;

@@ -150,14 +150,15 @@ __device__ __forceinline__ f32x4 w8_values(const i32x4 acc, const Channels& c, f
   return v;
 }
 
+__device__ __forceinline__ f32x4 w8_values_of(const i32x4 acc, const Channels& c, float s, int act) {
+  if (act == PH_ACT_RELU) return w8_values<PH_ACT_RELU>(acc, c, s);
+  if (act == PH_ACT_PRELU) return w8_values<PH_ACT_PRELU>(acc, c, s);
+  return w8_values<PH_ACT_NONE>(acc, c, s);
+}
 // one sum of four channels -> out
 template <typename O>
-__device__ __forceinline__ void w8_finish4(const PhW8Params& p, const i32x4 a, const Channels& c, unsigned m, int n, float s) {
-  f32x4 v;
-  if (p.act == PH_ACT_RELU) v = w8_values<PH_ACT_RELU>(a, c, s);
-  else if (p.act == PH_ACT_PRELU) v = w8_values<PH_ACT_PRELU>(a, c, s);
-  else v = w8_values<PH_ACT_NONE>(a, c, s);
-  w8_store4<O>((O*)p.out + ph_row_off(p.outr, m) + n, v, p.N - n);
+__device__ __forceinline__ void w8_finish4(const PhW8Params& p, const i32x4 a, unsigned m, int n, float s) {
+  w8_store4<O>((O*)p.out + ph_row_off(p.outr, m) + n, w8_values_of(a, w8_channels(p, n), s, p.act), p.N - n);
 }
 
 // A wave's TM x TN fragments -> out, tokens m0 + .. (s: the scales of a lane's tokens), channels n0 + ...  In a fragment the 16 lanes side by side hold 16

@@ -302,7 +302,7 @@ __global__ __launch_bounds__(64 * W) void w8_few_kernel(const PhW8Params p, cons
     const int n = nb * 16 + fq * 4;
     if (m >= p.M || n >= p.N) return;
     if (SPLIT) *(i32x4*)(p.parts + ((int64_t)blockIdx.y * p.M + m) * (p.nnb * 16) + n) = a;
-    else w8_finish4<O>(p, a, w8_channels(p, n), m, n, FLOAT ? s_scale[m] : p.qs[m]);
+    else w8_finish4<O>(p, a, m, n, FLOAT ? s_scale[m] : p.qs[m]);
   }
 }
 
@@ -324,7 +324,7 @@ __global__ __launch_bounds__(256) void w8_join_kernel(const PhW8Params p, int pa
 #pragma unroll
     for (int s = 0; s < 8; s++) a += b[s];
   }
-  w8_finish4<O>(p, a, w8_channels(p, n), m, n, p.qs[m]);
+  w8_finish4<O>(p, a, m, n, p.qs[m]);
 }
 
 template <int TM, bool SPLIT, typename O>

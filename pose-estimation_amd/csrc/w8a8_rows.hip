@@ -245,9 +245,9 @@ __global__ __launch_bounds__(512, 4) void w8_pair_kernel(const PhW8Pair p) {
 #pragma unroll
   for (int u = 0; u < U; u++) z[u] = i32x4{0, 0, 0, 0};
   const int n = nb2 * 16 + fq * 4;
-  PhW8Params o;
-  o.ws = p.ws2, o.bias = p.bias2, o.slope = p.slope2, o.act = p.act2, o.N = p.N, o.out = p.out, o.outr = p.outr;
-  const Channels c2 = w8_channels(o, min(n, p.nnb2 * 16 - 4));
+  const int at = min(n, p.nnb2 * 16 - 4);
+  const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+  const Channels c2 = {*(const f32x4*)(p.ws2 + at), p.bias2 ? *(const f32x4*)(p.bias2 + at) : zero, p.slope2 ? *(const f32x4*)(p.slope2 + at) : zero};
   const char* const wq = w2 + min(nb2, p.nnb2 - 1) * p.nkb2 * 1024 + lane * 16;
   for (int kb = 0; kb < p.nkb2; kb++) {
     const i32x4 w = *(const i32x4*)(wq + kb * 1024);
@@ -261,11 +261,22 @@ __global__ __launch_bounds__(512, 4) void w8_pair_kernel(const PhW8Pair p) {
   for (int u = 0; u < U; u++) {
     const int i = t0 + u * dt;
     const unsigned m = m0 + i * 16 + fr;
-    if (i < TF && m < p.M && n < p.N && nb2 < p.nnb2) {
-      const float s = s2[i * 16 + fr];
-      if (p.out_type == PH_F32) w8_finish4<float>(o, z[u], c2, m, n, s);
-      else if (p.out_type == PH_F16) w8_finish4<_Float16>(o, z[u], c2, m, n, s);
-      else w8_finish4<bf16>(o, z[u], c2, m, n, s);
+    if (i >= TF || m >= p.M || n >= p.N || nb2 >= p.nnb2) continue;
+    const f32x4 v = w8_values_of(z[u], c2, s2[i * 16 + fr], p.act2);
+    for (int d = 0; d < p.n_out; d++) {
+      const PhW8Out& o = p.out[d];
+      const int64_t off = ph_row_off(o.r, m) + n * o.step;
+      if (o.step != 1) {   // planes of f32
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+          if (n + e < p.N) ((float*)o.p)[off + e * o.step] = v[e];
+      } else if (o.type == PH_F32) {
+        w8_store4<float>((float*)o.p + off, v, p.N - n);
+      } else if (o.type == PH_F16) {
+        w8_store4<_Float16>((_Float16*)o.p + off, v, p.N - n);
+      } else {
+        w8_store4<bf16>((bf16*)o.p + off, v, p.N - n);
+      }
     }
   }
 }

@@ -11,7 +11,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("POSEHIP_LIB") or os.path.join(os.path.dirname(_HERE), "lib", "libposehip.so")
 
 PH_MAX_DST = 8
-PH_OP_CONV, PH_OP_POOL = 0, 1
+PH_OP_CONV, PH_OP_POOL, PH_OP_CONV_W8A8 = 0, 1, 2
 PH_ACT_NONE, PH_ACT_RELU, PH_ACT_PRELU = 0, 1, 2
 PH_PRE_CV2, PH_PRE_NATIVE = 0, 1
 PH_NOALLOC_MAX_FRAMES = 8

@@ -12,6 +12,7 @@ runs batch 1) and the ``posehip_*`` keys of the params dict:
                            missing ``model_folder`` raises FileNotFoundError
   posehip_device         : GPU index (default 0)
   posehip_batch          : max frames per call (default 1)
+  posehip_w8a8           : the 1x1 layers that close a stage in 8-bit integers (default False)
 """
 import argparse
 import math
@@ -136,7 +137,8 @@ class Wrapper:
     def _ensure(self, net_w, net_h, batch):
         key = (net_w, net_h)
         if self._built is None or self._built[:2] != key or self._built[2] < batch:
-            plan = graph.build_plan(self._net, self._weights, height=net_h, width=net_w)
+            plan = graph.build_plan(self._net, self._weights, height=net_h, width=net_w,
+                                    w8a8=bool(self.params.get("posehip_w8a8", False)))
             cap = max(batch, int(self.params.get("posehip_batch", 1)))
             self._engine.build(plan, cap)
             self._built = (net_w, net_h, cap)
@@ -592,7 +594,7 @@ _FLAG_TO_PARAM = {"op_model_folder": "model_folder", "op_model_pose": "model_pos
                   "op_net_resolution": "net_resolution", "op_heatmaps_add_parts": "heatmaps_add_parts",
                   "op_heatmaps_add_bkg": "heatmaps_add_bkg", "op_heatmaps_add_PAFs": "heatmaps_add_PAFs",
                   "op_heatmaps_scale": "heatmaps_scale"}
-_POSEHIP_FLAGS = ("posehip_random_weights", "posehip_device", "posehip_batch")
+_POSEHIP_FLAGS = ("posehip_random_weights", "posehip_device", "posehip_batch", "posehip_w8a8")
 
 
 class OpenPosePoseExtractor:

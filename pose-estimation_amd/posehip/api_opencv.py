@@ -50,11 +50,14 @@ class PyOpenPoseOpenCV:
         self._weights = None
         self._batch = 0
         self._last_b = 0
+        self._w8a8 = False
 
     def load(self, proto_file: str, weights_file: str, cuda: bool = True, random_weights: Optional[int] = None,
-             device: int = 0) -> None:
+             device: int = 0, w8a8: bool = False) -> None:
         """Loads the Caffe model (``readNetFromCaffe``, skeleton.py:39-53).  ``cuda``
-        is accepted for compatibility; the network always runs on the MI355X."""
+        is accepted for compatibility; the network always runs on the MI355X.  w8a8: the 1x1 layers that close a
+        stage in 8-bit integers."""
+        self._w8a8 = bool(w8a8)
         if os.path.exists(proto_file):
             with open(proto_file) as f:
                 self._parsed = caffe_io.parse_prototxt(f.read())
@@ -75,7 +78,8 @@ class PyOpenPoseOpenCV:
 
     def _ensure(self, batch):
         if batch > self._batch:
-            plan = graph.build_plan(self._parsed, self._weights, height=self.image_height, width=self.image_width)
+            plan = graph.build_plan(self._parsed, self._weights, height=self.image_height, width=self.image_width,
+                                    w8a8=self._w8a8)
             self.net.engine.build(plan, batch)
             self._batch = batch
 

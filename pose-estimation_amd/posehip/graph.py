@@ -63,7 +63,7 @@ class Plan:
         keep = []
         for i, o in enumerate(self.ops):
             d = ops[i]
-            d.type = o["type"]
+            d.type = _ffi.PH_OP_CONV_W8A8 if o.get("w8a8") else o["type"]
             d.in_buf, d.in_coff, d.cin_read = o["in_buf"], o["in_coff"], o["cin_read"]
             d.kh = d.kw = o["k"]
             d.cout, d.act = o["cout"], o["act"]
@@ -201,8 +201,25 @@ def _build_nodes(net, height, width):
     return nodes, inp, last
 
 
-def build_plan(net, weights, height=None, width=None, tile_overrides=None, fuse_pool=True):
-    """net: parsed prototxt; weights: {layer name: [blobs]}."""
+def _mark_w8a8(plan):
+    """Pairs of 1x1 layers that the 8-bit kernel takes (PH_OP_CONV_W8A8): the first one's output read by the second only,
+    at most 512 -> 512 -> 64 channels."""
+    readers = {}
+    for o in plan.ops:
+        readers[o["in_buf"]] = readers.get(o["in_buf"], 0) + 1
+    for a, b in zip(plan.ops, plan.ops[1:]):
+        if a["type"] != _ffi.PH_OP_CONV or b["type"] != _ffi.PH_OP_CONV or a["k"] != 1 or b["k"] != 1 or a.get("w8a8"):
+            continue
+        if len(a["dst"]) != 1 or a["f32_coff"] >= 0 or a["dst"][0] != (b["in_buf"], b["in_coff"]):
+            continue
+        if readers[b["in_buf"]] != 1 or a["cin_read"] > 512 or a["cout"] > 512 or b["cin_read"] > 512 or b["cout"] > 64:
+            continue
+        a["w8a8"] = b["w8a8"] = True
+
+
+def build_plan(net, weights, height=None, width=None, tile_overrides=None, fuse_pool=True, w8a8=False):
+    """net: parsed prototxt; weights: {layer name: [blobs]}.  w8a8: the pairs of 1x1 layers that close a stage run in
+    8-bit integers (a scale per pixel and per output channel) where they fit; everything else stays bf16."""
     nodes, inp, out = _build_nodes(net, height, width)
     plan = Plan()
     plan.in_h, plan.in_w = inp.h, inp.w
@@ -320,6 +337,8 @@ def build_plan(net, weights, height=None, width=None, tile_overrides=None, fuse_
                                  cin_read=plan.bufs[b]["channels"], k=2, cout=n.cout, act=0,
                                  dst=list(n.views), f32_coff=-1, h=n.h, w=n.w))
             plan.op_names.append(n.name)
+    if w8a8:
+        _mark_w8a8(plan)
     return plan
 
 

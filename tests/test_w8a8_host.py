@@ -121,3 +121,18 @@ def test_output_rows_that_overlap_are_refused():
         with pytest.raises(ValueError):
             w8a8._out_rows(x.shape, x.stride(), torch.Size((4, 6)), out.stride())
     w8a8._out_rows(x.shape, x.stride(), torch.Size((4, 6)), torch.empty(4, 9)[:, 2:8].stride())
+
+
+def test_plans_mark_the_pairs_that_fit():
+    from posehip import caffe_io, graph
+    for proto, pairs in ((caffe_io.body25_prototxt(64, 96), 6), (caffe_io.coco_prototxt(64, 96), 12)):
+        net = caffe_io.parse_prototxt(proto)
+        weights = graph.random_weights(net, seed=0)
+        plan = graph.build_plan(net, weights)
+        assert not any(o.get("w8a8") for o in plan.ops)
+        plan8 = graph.build_plan(net, weights, w8a8=True)
+        marked = [i for i, o in enumerate(plan8.ops) if o.get("w8a8")]
+        assert len(marked) == 2 * pairs and all(b == a + 1 for a, b in zip(marked[::2], marked[1::2]))
+        assert all(plan8.ops[i]["k"] == 1 for i in marked) and plan8.flops_per_frame() == plan.flops_per_frame()
+        types = [d.type for d in plan8.to_ctypes()[1]]
+        assert types.count(_ffi.PH_OP_CONV_W8A8) == 2 * pairs and [d.type for d in plan.to_ctypes()[1]].count(2) == 0
