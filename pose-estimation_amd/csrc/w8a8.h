@@ -30,7 +30,7 @@ struct PhW8Params {
   const float* slope;    // [N16] or NULL
   int act;
   int stream;            // store past the caches
-  int loose;             // rows start anywhere (ph_w8_loose() says whether the product takes that)
+  int loose;             // rows start anywhere (ph_w8_choose_loose())
   unsigned M;
   int N, K, nkb, nnb;    // nkb = K128 / 64 fragments along K (even), nnb = N16 / 16 along N
   void* out;
@@ -43,7 +43,7 @@ struct PhW8Choice {
   int kernel, parts;
 };
 PhW8Choice ph_w8_choose(int64_t M, int N, int nkb);
-bool ph_w8_loose(int64_t M, int K, int N);
+PhW8Choice ph_w8_choose_loose(int64_t M, int K, int N);   // kernel < 0: none takes them
 int64_t ph_w8_parts_bytes(const PhW8Choice& c, int64_t M, int N);
 int ph_launch_w8_product(const PhW8Params& p, const PhW8Choice& c, int out_type, hipStream_t st);
 

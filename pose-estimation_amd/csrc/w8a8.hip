@@ -350,7 +350,7 @@ int64_t ph_w8_workspace(int op, int64_t m, int k, int h, int n) {
   if (m == 0) return 0;
   switch (op) {
     case PH_W8_MATMUL: return RowsSpace(nullptr, m, k, n, false, false).used();
-    case PH_W8_MATMUL_ANY: return RowsSpace(nullptr, m, k, n, !ph_w8_loose(m, k, n), false).used();
+    case PH_W8_MATMUL_ANY: return RowsSpace(nullptr, m, k, n, ph_w8_choose_loose(m, k, n).kernel < 0, false).used();
     case PH_W8_LINEAR: return linear_space(m, k, n);
     case PH_W8_FEED_FORWARD:
       if (h < 1) {
@@ -380,7 +380,9 @@ int ph_w8_matmul(int device, void* stream, const int8_t* q, const ph_rows* rows,
   ph_rows orow = *rows;
   for (int d = 0; d < 3; d++) orow.stride[d] = out_stride[d];
   PhRowMap qr = row_map(*rows);
-  const bool even = aligned16(q, qr), direct = even || ph_w8_loose(M, layer->k, layer->n);
+  const bool even = aligned16(q, qr);
+  const PhW8Choice any = even ? PhW8Choice{-1, 1} : ph_w8_choose_loose(M, layer->k, layer->n);
+  const bool direct = even || any.kernel >= 0;
   const RowsSpace w(ws, M, layer->k, layer->n, !direct, false);
   if (!ws_ok(who, ws, ws_bytes, w.used())) return -3;
   W8_DEVICE(device);
@@ -394,7 +396,7 @@ int ph_w8_matmul(int device, void* stream, const int8_t* q, const ph_rows* rows,
   }
   PhW8Params p = product_params(q, qr, scale, (unsigned)M, *layer, out, row_map(orow), w.parts, out_type);
   p.loose = direct && !even;
-  return ph_launch_w8_product(p, w.choice, out_type, (hipStream_t)stream);
+  return ph_launch_w8_product(p, p.loose ? any : w.choice, out_type, (hipStream_t)stream);
 }
 
 int ph_w8_linear(int device, void* stream, const void* x, int x_type, const ph_rows* rows, const ph_w8_layer* layer, void* out,

@@ -164,7 +164,8 @@ static int launch_tile(const PhW8Params& p, int parts, hipStream_t st) {
 
 // ---- product: few tokens -------------------------------------------------------------------------------------------------
 //
-// Up to 64 tokens: the weights are read once, each fragment by one wave straight into registers (a fragment is 1 KiB in
+// Up to 64 tokens (and more, 64 to a block, where rows of any alignment would have to be laid out anew first): the weights
+// are read once, each fragment by one wave straight into registers (a fragment is 1 KiB in
 // one piece), and the rows, which every block needs, come from cache.  A block has 16 channels; its waves take fragments
 // along K in turn and their sums meet in LDS.
 //
@@ -247,6 +248,7 @@ __global__ __launch_bounds__(64 * W) void w8_few_kernel(const PhW8Params p, cons
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int fr = lane & 15, fq = lane >> 4;
   const int nb = blockIdx.x;
+  const unsigned m0 = blockIdx.z * (16 * TM);
   const int kb0 = SPLIT ? (int)((int64_t)p.nkb * blockIdx.y / gridDim.y) : 0;
   const int kb1 = SPLIT ? (int)((int64_t)p.nkb * (blockIdx.y + 1) / gridDim.y) : p.nkb;
   const int8_t* const wp = p.w + (int64_t)nb * p.nkb * 1024 + lane * 16;
@@ -263,7 +265,7 @@ __global__ __launch_bounds__(64 * W) void w8_few_kernel(const PhW8Params p, cons
   int xq[TM];   // FLOAT: in LDS
 #pragma unroll
   for (int i = 0; i < TM; i++) {
-    const unsigned m = min((unsigned)(i * 16 + fr), p.M - 1);
+    const unsigned m = min(m0 + i * 16 + fr, p.M - 1);
     xp[i] = FLOAT ? nullptr : p.q + ph_row_off(p.qr, m);
     xq[i] = (int)m * pitch;
   }
@@ -298,7 +300,7 @@ __global__ __launch_bounds__(64 * W) void w8_few_kernel(const PhW8Params p, cons
     i32x4 a = *(const i32x4*)&red[0][wave][lane * 4];
 #pragma unroll
     for (int w = 1; w < W; w++) a += *(const i32x4*)&red[w][wave][lane * 4];
-    const unsigned m = wave * 16 + fr;
+    const unsigned m = m0 + wave * 16 + fr;
     const int n = nb * 16 + fq * 4;
     if (m >= p.M || n >= p.N) return;
     if (SPLIT) *(i32x4*)(p.parts + ((int64_t)blockIdx.y * p.M + m) * (p.nnb * 16) + n) = a;
@@ -329,7 +331,7 @@ __global__ __launch_bounds__(256) void w8_join_kernel(const PhW8Params p, int pa
 
 template <int TM, bool SPLIT, typename O>
 static int launch_few(const PhW8Params& p, int parts, hipStream_t st) {
-  hipLaunchKernelGGL((w8_few_kernel<TM, 8, SPLIT, int8_t, O>), dim3(p.nnb, SPLIT ? parts : 1), dim3(512), 0, st, p, FloatRows{});
+  hipLaunchKernelGGL((w8_few_kernel<TM, 8, SPLIT, int8_t, O>), dim3(p.nnb, SPLIT ? parts : 1, (p.M - 1) / (16 * TM) + 1), dim3(512), 0, st, p, FloatRows{});
   PH_CHECK(hipGetLastError());
   return 0;
 }
@@ -380,8 +382,12 @@ PhW8Choice ph_w8_choose(int64_t M, int N, int nkb) {
   return best;
 }
 
-bool ph_w8_loose(int64_t M, int K, int N) {
-  return K >= 16 && M <= 64 && ph_w8_choose(M, N, (int)((K + 127) / 128 * 2)).kernel == K_FEW;
+// Rows of any alignment: the few-token kernel takes them as they are, also for more tokens as long as its blocks' reading
+// of all rows (from cache) costs less than a launch that lays them out anew: 267 x 546 -> 2611 XX us, else 8.4.
+PhW8Choice ph_w8_choose_loose(int64_t M, int K, int N) {
+  const PhW8Choice c = ph_w8_choose(M, N, (K + 127) / 128 * 2);
+  if (K < 16 || (M <= 64 && c.kernel != K_FEW) || (M > 64 && (double)M * K * ((N + 15) / 16) > 3e6)) return {-1, 1};
+  return M <= 64 ? c : PhW8Choice{K_FEW, 1};
 }
 
 int64_t ph_w8_parts_bytes(const PhW8Choice& c, int64_t M, int N) {
