@@ -78,8 +78,8 @@ def test_c_refusals():
     assert m(layer=layer(n=0)) == -1 and m(layer=layer(k=w8a8.MAX_K + 1)) == -1 and m(layer=layer(act=3)) == -1
     assert m(layer=layer(act=2)) == -1 and m(layer=None) == -1 and m(t=9) == -1 and m(q=None) == -1 and m(s=None) == -1
     assert m(out=None) == -1 and m(st=None) == -1 and m(rows=None) == -1
-    r = rows((1, 1, 100))
-    assert m(q=4097, rows=r) == -3 and m(rows=rows((1, 1, 100), (0, 0, 65))) == -3 and m(q=4097, rows=r, ws=4096 + 16, nws=1 << 20) == -3
+    r = rows((1, 1, 100000))
+    assert m(q=4097, rows=r) == -3 and m(rows=rows((1, 1, 100000), (0, 0, 65))) == -3 and m(q=4097, rows=r, ws=4096 + 16, nws=1 << 20) == -3
     assert b"workspace" in lib.ph_last_error()
     li = lambda **k: lib.ph_w8_linear(0, None, k.get("x", 4096), k.get("t", 0), k.get("rows", rows((1, 1, 100))), layer(k=4000), 4096, k.get("ot", 0),   # noqa: E731
                                       st, k.get("ws", 4096), k.get("nws", 1 << 20))
