@@ -297,13 +297,14 @@ int ph_decode_v1_walks(ph_ctx* ctx, int32_t* wave, int32_t* group);
 #define PH_F16 1
 #define PH_BF16 2
 /* Rows in three nested dimensions (of size 1 where there are fewer), strides in elements, any stride (0 too) for inputs;
- * the values of a row are consecutive.  At most 2^31 - 1 rows. */
+ * the values of a row are consecutive.  At most 2^31 - 1 rows, and no more than a launch's 2^32 threads hold (tens of
+ * millions of short rows, 4 million of more than 8192 values): a call of more fails with -1. */
 typedef struct {
   int64_t n[3];
   int64_t stride[3];
 } ph_rows;
 /* A layer: n output channels, k inputs (k <= 131071: the int32 sum cannot overflow; n <= 2^20).  scale / bias / slope
- * hold n values rounded up to a multiple of 16; bias may be NULL, slope may be NULL unless act is PH_ACT_PRELU. */
+ * hold n values rounded up to a multiple of 16, each array 16-byte aligned; bias may be NULL, slope may be NULL unless act is PH_ACT_PRELU. */
 typedef struct {
   const int8_t* packed; /* ph_w8_pack's output */
   const float* scale;

@@ -20,6 +20,14 @@ __host__ __device__ static inline int64_t ph_row_off(const PhRowMap& r, unsigned
   return (int64_t)i0 * r.s0 + (int64_t)i1 * r.s1 + (int64_t)i2 * r.s2;
 }
 
+// A launch holds fewer than 2^32 threads: a call of more rows than that is refused.
+static inline int ph_w8_launchable(int64_t blocks, int64_t threads) {
+  if (blocks * threads <= 0xff000000ll) return 0;   // (counts rounded up to whole blocks still fit)
+  ph_set_error("8-bit layer: %lld blocks of %lld threads are more than a launch holds: take the rows in parts",
+               (long long)blocks, (long long)threads);
+  return -1;
+}
+
 struct PhW8Params {
   const int8_t* q;       // 8-bit rows, K contiguous values each (rows 16-byte aligned, unless loose)
   PhRowMap qr;

@@ -70,6 +70,7 @@ static int launch_quantize_t(const T* x, const PhRowMap& xr, unsigned M, int K, 
   int g = 0;
   while (g < 5 && groups[g] * 32 < K) g++;
   while (g < 5 && groups[g] * 8 < K && (int64_t)M * groups[g] < 64 * 4096) g++;
+  if (ph_w8_launchable(M, groups[g])) return -1;
 #define PH_Q(G)                                                                                                            \
   hipLaunchKernelGGL((quantize_rows_kernel<T, G, 4>), dim3(G <= 64 ? (M - 1) / (G <= 64 ? 256 / G : 1) + 1 : M),              \
                      dim3(G <= 64 ? 256 : G), 0, st, x, xr, M, K, q, pitch, scale);                                         \
@@ -200,9 +201,10 @@ bool rows_ok(const char* who, const ph_rows* r, int64_t& M) {
 }
 
 bool layer_ok(const char* who, const ph_w8_layer* l) {
-  if (!l || !l->packed || !l->scale || l->n < 1 || l->n > W8_MAX_N || l->k < 1 || l->k > W8_MAX_K ||
+  const uintptr_t at = l ? (uintptr_t)l->packed | (uintptr_t)l->scale | (uintptr_t)l->bias | (uintptr_t)l->slope : 0;
+  if (!l || !l->packed || !l->scale || (at & 15) || l->n < 1 || l->n > W8_MAX_N || l->k < 1 || l->k > W8_MAX_K ||
       l->act < PH_ACT_NONE || l->act > PH_ACT_PRELU || (l->act == PH_ACT_PRELU && !l->slope)) {
-    ph_set_error("%s: bad layer (1 <= n <= %d, 1 <= k <= %d, PReLU needs slopes)", who, W8_MAX_N, W8_MAX_K);
+    ph_set_error("%s: bad layer (1 <= n <= %d, 1 <= k <= %d, PReLU needs slopes, arrays 16-byte aligned)", who, W8_MAX_N, W8_MAX_K);
     return false;
   }
   return true;
@@ -321,6 +323,7 @@ int ph_w8_pack(int device, void* stream, const int8_t* w, int64_t row_stride, in
   W8_DEVICE(device);
   const int nkb = nkb_of(k), nnb = (n + 15) / 16;
   const int64_t pieces = (int64_t)nkb * nnb * 64;
+  if (ph_w8_launchable(pieces, 1)) return -1;
   hipLaunchKernelGGL(pack_weight_kernel, dim3((unsigned)((pieces + 255) / 256)), dim3(256), 0, (hipStream_t)stream, w,
                      row_stride, n, k, nkb, nnb, packed);
   PH_CHECK(hipGetLastError());
@@ -388,6 +391,7 @@ int ph_w8_matmul(int device, void* stream, const int8_t* q, const ph_rows* rows,
   W8_DEVICE(device);
   if (!direct) {
     const int64_t pitch = q_pitch_of(layer->k), threads = M * ((pitch + 63) / 64);
+    if (ph_w8_launchable(threads, 1)) return -1;
     hipLaunchKernelGGL(repitch_kernel, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, (hipStream_t)stream, q, qr,
                        (unsigned)M, layer->k, w.q, pitch);
     PH_CHECK(hipGetLastError());

@@ -156,7 +156,8 @@ static int launch_tile(const PhW8Params& p, int parts, hipStream_t st) {
   static int granted[PH_MAX_DEVICES];
   const void* fn = (const void*)w8_tile_kernel<BM, BN, WM, WN, NST, SPLIT, O>;
   if (lds > 64 * 1024 && ph_ensure_lds(fn, lds, granted)) return -1;
-  const unsigned mt = (p.M + BM - 1) / BM, nt = (p.N + BN - 1) / BN;
+  const unsigned mt = (p.M - 1) / BM + 1, nt = (p.N - 1) / BN + 1;
+  if (ph_w8_launchable((int64_t)mt * nt * parts, 64 * WM * WN)) return -1;
   hipLaunchKernelGGL((w8_tile_kernel<BM, BN, WM, WN, NST, SPLIT, O>), dim3(mt * nt, SPLIT ? parts : 1), dim3(64 * WM * WN), lds, st, p, mt, nt);
   PH_CHECK(hipGetLastError());
   return 0;
@@ -416,6 +417,7 @@ static int launch_product_t(const PhW8Params& p, const PhW8Choice& c, hipStream_
   if (c.parts == 1) return launch_kernel<false, O>(p, c, st);
   if (launch_kernel<true, O>(p, c, st)) return -1;
   const int64_t pieces = (int64_t)p.M * ((p.N + 3) / 4);
+  if (ph_w8_launchable(pieces, 1)) return -1;
   hipLaunchKernelGGL((w8_join_kernel<O>), dim3((unsigned)((pieces + 255) / 256)), dim3(256), 0, st, p, c.parts);
   PH_CHECK(hipGetLastError());
   return 0;

@@ -117,6 +117,7 @@ static int launch_rows_f(const PhW8Params& p, const FloatRows& f, hipStream_t st
   constexpr int lds = BT * 4 + 12 * 64 * WN + (rows > tile ? rows : tile);   // <= 76 KB: two blocks a CU
   static int granted[PH_MAX_DEVICES];
   if (lds > 64 * 1024 && ph_ensure_lds((const void*)w8_rows_kernel<TF, WN, T, O>, lds, granted)) return -1;
+  if (ph_w8_launchable((int64_t)((p.M - 1) / BT + 1) * ((p.N - 1) / (64 * WN) + 1), 512)) return -1;
   hipLaunchKernelGGL((w8_rows_kernel<TF, WN, T, O>), dim3((p.M - 1) / BT + 1, (p.N - 1) / (64 * WN) + 1), dim3(512), lds, st, p, f);
   PH_CHECK(hipGetLastError());
   return 0;
@@ -289,6 +290,7 @@ static int launch_pair_f(const PhW8Pair& p, hipStream_t st) {
   const int lds = BT * PITCH + 10 * BT * 4 + 12 * PAIR_MAX + p.nnb2 * p.nkb2 * 1024;   // <= 74 KB: two blocks a CU
   static int granted[PH_MAX_DEVICES];
   if (lds > 64 * 1024 && ph_ensure_lds((const void*)w8_pair_kernel<TF, ACT, T>, lds, granted)) return -1;
+  if (ph_w8_launchable((p.M - 1) / BT + 1, 512)) return -1;
   hipLaunchKernelGGL((w8_pair_kernel<TF, ACT, T>), dim3((p.M - 1) / BT + 1), dim3(512), lds, st, p);
   PH_CHECK(hipGetLastError());
   return 0;

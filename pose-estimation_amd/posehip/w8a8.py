@@ -20,7 +20,9 @@ gives NaN outputs and touches no other row.  There are no gradients: tensors tha
 
 Tensors are CUDA tensors of f32 / f16 / bf16 with the values of a row consecutive (last stride 1) and any other strides;
 leading dimensions that do not merge into three are refused.  Work is put on torch's current stream of the tensors'
-device, waits for nothing, and can be captured into a graph.  All arithmetic happens in libposehip.so.
+device, waits for nothing, and can be captured into a graph; a tensor (a layer's weights among them) that is used on
+another stream than the one it was made on has to stay alive until that stream is done with it, as with any torch
+operation.  All arithmetic happens in libposehip.so.
 """
 import ctypes as C
 from functools import lru_cache
@@ -247,6 +249,8 @@ def matmul(q, scale, layer, out=None, dtype=None):
         raise ValueError(f"q must be a CUDA int8 tensor [.., {layer.k}], got {q.dtype} {tuple(q.shape)} on {q.device}")
     if scale.shape != q.shape[:-1] or scale.dtype != torch.float32 or scale.device != q.device:
         raise ValueError(f"scale must be f32 {tuple(q.shape[:-1])} on {q.device}, got {scale.dtype} {tuple(scale.shape)} on {scale.device}")
+    if scale.requires_grad and torch.is_grad_enabled():
+        raise ValueError("8-bit layers have no gradient: call them under torch.no_grad() or detach their inputs")
     if not scale.is_contiguous():
         scale = scale.contiguous()
     y, rows, ostride, m = _output(q, layer.n, out, dtype, torch.bfloat16)

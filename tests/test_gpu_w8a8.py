@@ -230,6 +230,52 @@ def test_feed_forward(w8, M, K, H, N, t, out, act):
     assert torch.equal(torch.nan_to_num(y.float()), torch.nan_to_num(z.float()))
 
 
+# where one kernel hands over to another: row lengths, tokens, channels
+@pytest.mark.parametrize("M,K,N", [(64, 512, 300), (65, 512, 300), (64, 513, 40), (65, 513, 40), (2, 16384, 20), (2, 16385, 20), (100, 7, 40),
+                                   (64, 7, 40), (70, 8, 64), (70, 9, 65), (8192, 64, 130), (8193, 64, 130), (8193, 8, 520),
+                                   (8200, 512, 260), (8200, 129, 60), (8200, 384, 128), (8200, 385, 129), (300, 100, 4096),
+                                   (300, 100, 4097), (8200, 40, 2049)])
+def test_linear_borders(w8, M, K, N):
+    rng = np.random.default_rng(M * 3 + K * 5 + N)
+    w, ws, bias, slope = weights(rng, N, K)
+    layer = make(w8, w, ws, bias, "prelu", slope)
+    for t, out in (("bf16", "bf16"), ("f32", "f32")):
+        x = rows(rng, M, K, t).cuda()
+        x[M // 3, K // 2] = float("nan")
+        wide = torch.zeros(M, K + 3, dtype=x.dtype, device="cuda")
+        wide[:, 3:] = x
+        y = w8.linear(x, layer, dtype=TYPES[out])
+        z = w8.linear(wide[:, 3:], layer, dtype=TYPES[out])   # rows that start at odd places
+        assert torch.equal(y.view(torch.uint8), z.view(torch.uint8))
+        same(y, ref.linear(x.double().cpu().numpy(), w, ws, bias, "prelu", slope))
+
+
+@pytest.mark.parametrize("M,K,H,N", [(20000, 24, 40, 20), (20001, 24, 40, 20), (20001, 512, 512, 64), (130, 512, 512, 65), (130, 513, 512, 64),
+                                     (130, 512, 513, 64), (130, 7, 64, 16), (130, 8, 1, 1), (33, 500, 17, 33), (64, 96, 500, 48)])
+def test_feed_forward_borders(w8, M, K, H, N):
+    rng = np.random.default_rng(M + 7 * K + H + N)
+    a, b = weights(rng, H, K), weights(rng, N, H)
+    x = rows(rng, M, K, "f16").cuda()
+    x[M // 2, 0] = float("inf")
+    l1, l2 = make(w8, a[0], a[1], a[2], "relu"), make(w8, b[0], b[1], b[2], "prelu", b[3])
+    y = w8.feed_forward(x, l1, l2, dtype=torch.float32)
+    same(y, ref.feed_forward(x.double().cpu().numpy(), (a[0], a[1], a[2], "relu"), (b[0], b[1], b[2], "prelu", b[3])))
+
+
+@pytest.mark.parametrize("M,K,N", [(1, 15, 20), (1, 16, 20), (5, 17, 33), (64, 31, 100), (65, 33, 100), (64, 4099, 100), (200, 47, 70), (3, 40001, 5),
+                                   (700, 1001, 90), (64, 64, 64)])
+def test_matmul_of_rows_that_start_anywhere(w8, M, K, N):
+    """Nothing behind the last row's end is read: the storage ends there, and what stands before and between is noise."""
+    rng = np.random.default_rng(K + M)
+    w, ws, bias, _ = weights(rng, N, K)
+    layer = make(w8, w, ws, bias)
+    s = torch.rand(M, device="cuda")
+    for gap, lead in ((0, 0), (1, 5), (7, 3)):
+        store = torch.from_numpy(rng.integers(-127, 128, lead + (M - 1) * (K + gap) + K).astype(np.int8)).cuda()
+        q = store.as_strided((M, K), (K + gap, 1), lead)
+        same(w8.matmul(q, s, layer, dtype=torch.float32), ref.matmul(q.cpu().numpy(), s.cpu().numpy(), w, ws, bias))
+
+
 def test_long_offsets(w8):
     """Rows behind the first 2^31 and 2^32 elements, of the input and of the output."""
     M, K = 70001, 65536
@@ -366,6 +412,43 @@ def test_same_results_every_time(w8):
     for _ in range(5):
         assert torch.equal(w8.linear(x, layer), y)
     same(y, ref.linear(x.double().cpu().numpy(), w, ws, bias))
+
+
+def test_first_calls_inside_a_capture(w8):
+    """Nothing that a first call sets up needs a call outside of a capture."""
+    rng = np.random.default_rng(12)
+    a, b = weights(rng, 500, 300), weights(rng, 33, 500)
+    l1, l2, l3 = make(w8, a[0], a[1], a[2], "relu"), make(w8, b[0], b[1], b[2]), make(w8, *weights(rng, 600, 2000)[:2])
+    x, v = rows(rng, 21000, 300, "f16"), rows(rng, 400, 2000, "f32")
+    dx, dv = x.cuda(), v.cuda()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        o = (w8.feed_forward(dx, l1, l2, dtype=torch.float16), w8.linear(dx, l1, dtype=torch.float16), w8.linear(dv, l3, dtype=torch.float16))
+    for _ in range(3):
+        g.replay()
+        e = (w8.feed_forward(dx, l1, l2), w8.linear(dx, l1), w8.linear(dv, l3, dtype=torch.float16))
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, r) for p, r in zip(o, e))
+
+
+def test_more_rows_than_a_launch_holds(w8):
+    """Refused before anything is launched."""
+    import ctypes as C
+    from posehip import _ffi
+    lib, buf = _ffi.lib(), torch.zeros(1 << 20, dtype=torch.uint8, device="cuda")
+    n = (1 << 31) - 1
+    r = _ffi.PhRows((C.c_int64 * 3)(1, 1, n), (C.c_int64 * 3)(0, 0, 0))
+    st = torch.cuda.current_stream().cuda_stream
+    assert lib.ph_w8_quantize_rows(0, st, buf.data_ptr(), _ffi.PH_F32, r, 300, buf.data_ptr(), 304, buf.data_ptr()) == -1
+    assert b"launch" in lib.ph_last_error()
+    rng = np.random.default_rng(0)
+    layer = make(w8, *weights(rng, 16, 64)[:2])
+    os = (C.c_int64 * 3)(0, 0, 16)
+    assert lib.ph_w8_matmul(0, st, buf.data_ptr(), r, buf.data_ptr(), layer.desc, buf.data_ptr(), 0, os, None, 0) == -1
+    assert lib.ph_w8_linear(0, st, buf.data_ptr(), 0, r, layer.desc, buf.data_ptr(), 0, os, None, 0) == -1
+    torch.cuda.synchronize()
+    assert not buf.any()
 
 
 def test_refusals(w8):

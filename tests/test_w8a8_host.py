@@ -78,6 +78,9 @@ def test_c_refusals():
     assert m(layer=layer(n=0)) == -1 and m(layer=layer(k=w8a8.MAX_K + 1)) == -1 and m(layer=layer(act=3)) == -1
     assert m(layer=layer(act=2)) == -1 and m(layer=None) == -1 and m(t=9) == -1 and m(q=None) == -1 and m(s=None) == -1
     assert m(out=None) == -1 and m(st=None) == -1 and m(rows=None) == -1
+    odd = layer()
+    odd.scale = 4104
+    assert m(layer=odd) == -1
     r = rows((1, 1, 100000))
     assert m(q=4097, rows=r) == -3 and m(rows=rows((1, 1, 100000), (0, 0, 65))) == -3 and m(q=4097, rows=r, ws=4096 + 16, nws=1 << 20) == -3
     assert b"workspace" in lib.ph_last_error()
