@@ -304,7 +304,8 @@ typedef struct {
   int64_t stride[3];
 } ph_rows;
 /* A layer: n output channels, k inputs (k <= 131071: the int32 sum cannot overflow; n <= 2^20).  scale / bias / slope
- * hold n values rounded up to a multiple of 16, each array 16-byte aligned; bias may be NULL, slope may be NULL unless act is PH_ACT_PRELU. */
+ * hold n values rounded up to a multiple of 16, each array 16-byte aligned; bias may be NULL, slope may be NULL unless act
+ * is PH_ACT_PRELU. */
 typedef struct {
   const int8_t* packed; /* ph_w8_pack's output */
   const float* scale;
@@ -316,8 +317,8 @@ typedef struct {
  * bytes apart) into the order in which the matrix instructions take it; once per weight */
 int64_t ph_w8_packed_bytes(int n, int k);
 int ph_w8_pack(int device, void* stream, const int8_t* w, int64_t row_stride, int n, int k, int8_t* packed);
-/* x: f32 / f16 / bf16 rows -> q int8 [rows][q_pitch] (16-byte aligned, q_pitch a multiple of 16 and >= k; bytes from k
- * on are not meant for reading), scale f32 [rows] */
+/* x: f32 / f16 / bf16 rows (k <= 2^30) -> q int8 [rows][q_pitch] (16-byte aligned, q_pitch a multiple of 16 and >= k; bytes
+ * from k on are not meant for reading), scale f32 [rows] */
 int ph_w8_quantize_rows(int device, void* stream, const void* x, int x_type, const ph_rows* rows, int k, int8_t* q,
                         int64_t q_pitch, float* scale);
 #define PH_W8_MATMUL 0

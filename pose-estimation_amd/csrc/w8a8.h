@@ -46,9 +46,10 @@ struct PhW8Params {
   int* parts;            // split along K: sums [part][M][N16]
 };
 
-// How a product is done: which kernel, and in how many parts along K.
+// How a product is done: which kernel, in how many parts along K, and what that is expected to take.
 struct PhW8Choice {
   int kernel, parts;
+  float us;
 };
 PhW8Choice ph_w8_choose(int64_t M, int N, int nkb);
 PhW8Choice ph_w8_choose_loose(int64_t M, int K, int N);   // kernel < 0: none takes them

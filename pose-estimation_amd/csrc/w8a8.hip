@@ -137,6 +137,7 @@ __global__ void repitch_kernel(const int8_t* __restrict__ q, PhRowMap qr, unsign
 
 #define W8_MAX_K 131071      // 128 * 128 * K < 2^31
 #define W8_MAX_N (1 << 20)
+#define W8_MAX_ROW (1 << 30)   // of quantised rows: indexes past a row's end by one step stay ints
 
 namespace {
 
@@ -145,9 +146,14 @@ struct DeviceScope {
   int prev = -1;
   bool ok = false;
   explicit DeviceScope(int device) {
-    if (hipGetDevice(&prev) != hipSuccess) return;
+    if (hipGetDevice(&prev) != hipSuccess) {
+      prev = -1;
+      (void)hipGetLastError();
+      return;
+    }
     if (prev == device) prev = -1, ok = true;
     else ok = hipSetDevice(device) == hipSuccess;
+    if (!ok) (void)hipGetLastError();   // (else the next call's check of its launch would find it)
   }
   ~DeviceScope() {
     if (prev >= 0) (void)hipSetDevice(prev);
@@ -267,11 +273,10 @@ struct Pieces {
 // The workspace of one product: its parts' sums, 8-bit rows and their scales, as far as the call needs them.
 struct RowsSpace {
   Pieces w;
-  PhW8Choice choice;
   int* parts;
   int8_t* q = nullptr;
   float* s = nullptr;
-  RowsSpace(void* ws, int64_t M, int K, int N, bool rows, bool scales) : w{(char*)ws}, choice(ph_w8_choose(M, N, nkb_of(K))) {
+  RowsSpace(void* ws, const PhW8Choice& choice, int64_t M, int K, int N, bool rows, bool scales) : w{(char*)ws} {
     parts = (int*)w.take<char>(ph_w8_parts_bytes(choice, M, N));
     if (rows) q = w.take<int8_t>(M * q_pitch_of(K));
     if (scales) s = w.take<float>(M);
@@ -280,7 +285,24 @@ struct RowsSpace {
 };
 // rows of a layer that quantises them itself need no space
 bool itself(int64_t M, int K, int N) { return ph_w8_few_float(M, K) || ph_w8_rows_fit(M, K, N); }
-int64_t linear_space(int64_t M, int K, int N) { return itself(M, K, N) ? 0 : RowsSpace(nullptr, M, K, N, true, true).used(); }
+int64_t linear_space(int64_t M, int K, int N) {
+  return itself(M, K, N) ? 0 : RowsSpace(nullptr, ph_w8_choose(M, N, nkb_of(K)), M, K, N, true, true).used();
+}
+
+// How a product of given 8-bit rows is done, and whether they are laid out anew first.
+struct MatmulWay {
+  PhW8Choice choice;
+  bool anew, loose;
+  MatmulWay(int64_t M, int K, int N, bool even) {
+    anew = loose = false;
+    if (!even) {
+      choice = ph_w8_choose_loose(M, K, N);
+      loose = choice.kernel >= 0;
+      anew = !loose;
+    }
+    if (!loose) choice = ph_w8_choose(M, N, nkb_of(K));
+  }
+};
 
 int linear(const void* x, int x_type, const PhRowMap& xr, unsigned M, const ph_w8_layer& l, void* out, int out_type,
            const PhRowMap& outr, void* ws, hipStream_t st) {
@@ -289,10 +311,11 @@ int linear(const void* x, int x_type, const PhRowMap& xr, unsigned M, const ph_w
     const PhW8Params p = product_params(nullptr, xr, nullptr, M, l, out, outr, nullptr, out_type);
     return ph_w8_few_float(M, l.k) ? ph_launch_w8_few_float(p, f, x_type, out_type, st) : ph_launch_w8_rows(p, f, x_type, out_type, st);
   }
-  const RowsSpace w(ws, M, l.k, l.n, true, true);
+  const PhW8Choice choice = ph_w8_choose(M, l.n, nkb_of(l.k));
+  const RowsSpace w(ws, choice, M, l.k, l.n, true, true);
   const int64_t pitch = q_pitch_of(l.k);
   if (quantize(x, x_type, xr, M, l.k, w.q, pitch, w.s, st)) return -1;
-  return ph_launch_w8_product(product_params(w.q, even_rows(pitch), w.s, M, l, out, outr, w.parts, out_type), w.choice, out_type, st);
+  return ph_launch_w8_product(product_params(w.q, even_rows(pitch), w.s, M, l, out, outr, w.parts, out_type), choice, out_type, st);
 }
 
 // Of two layers: the inner rows in f32, and the larger of the two layers' spaces, one after the other in one place.
@@ -334,9 +357,9 @@ int ph_w8_quantize_rows(int device, void* stream, const void* x, int x_type, con
                         int64_t q_pitch, float* scale) {
   int64_t M;
   if (!rows_ok("ph_w8_quantize_rows", rows, M) || !type_ok("ph_w8_quantize_rows", x_type)) return -1;
-  if (k < 1 || q_pitch < q_pitch_of(k) || q_pitch % 16 || ((uintptr_t)q & 15)) {
-    ph_set_error("ph_w8_quantize_rows: k %d, q_pitch %lld: rows of 8-bit values are 16-byte aligned and hold k rounded up to 16",
-                 k, (long long)q_pitch);
+  if (k < 1 || k > W8_MAX_ROW || q_pitch < q_pitch_of(k) || q_pitch % 16 || ((uintptr_t)q & 15)) {
+    ph_set_error("ph_w8_quantize_rows: k %d, q_pitch %lld: 1 <= k <= 2^30, rows of 8-bit values are 16-byte aligned and hold k "
+                 "rounded up to 16", k, (long long)q_pitch);
     return -1;
   }
   if (M == 0) return 0;
@@ -352,8 +375,11 @@ int64_t ph_w8_workspace(int op, int64_t m, int k, int h, int n) {
   }
   if (m == 0) return 0;
   switch (op) {
-    case PH_W8_MATMUL: return RowsSpace(nullptr, m, k, n, false, false).used();
-    case PH_W8_MATMUL_ANY: return RowsSpace(nullptr, m, k, n, ph_w8_choose_loose(m, k, n).kernel < 0, false).used();
+    case PH_W8_MATMUL:
+    case PH_W8_MATMUL_ANY: {
+      const MatmulWay way(m, k, n, op == PH_W8_MATMUL);
+      return RowsSpace(nullptr, way.choice, m, k, n, way.anew, false).used();
+    }
     case PH_W8_LINEAR: return linear_space(m, k, n);
     case PH_W8_FEED_FORWARD:
       if (h < 1) {
@@ -384,12 +410,11 @@ int ph_w8_matmul(int device, void* stream, const int8_t* q, const ph_rows* rows,
   for (int d = 0; d < 3; d++) orow.stride[d] = out_stride[d];
   PhRowMap qr = row_map(*rows);
   const bool even = aligned16(q, qr);
-  const PhW8Choice any = even ? PhW8Choice{-1, 1} : ph_w8_choose_loose(M, layer->k, layer->n);
-  const bool direct = even || any.kernel >= 0;
-  const RowsSpace w(ws, M, layer->k, layer->n, !direct, false);
+  const MatmulWay way(M, layer->k, layer->n, even);
+  const RowsSpace w(ws, way.choice, M, layer->k, layer->n, way.anew, false);
   if (!ws_ok(who, ws, ws_bytes, w.used())) return -3;
   W8_DEVICE(device);
-  if (!direct) {
+  if (way.anew) {
     const int64_t pitch = q_pitch_of(layer->k), threads = M * ((pitch + 63) / 64);
     if (ph_w8_launchable(threads, 1)) return -1;
     hipLaunchKernelGGL(repitch_kernel, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, (hipStream_t)stream, q, qr,
@@ -399,8 +424,8 @@ int ph_w8_matmul(int device, void* stream, const int8_t* q, const ph_rows* rows,
     qr = even_rows(pitch);
   }
   PhW8Params p = product_params(q, qr, scale, (unsigned)M, *layer, out, row_map(orow), w.parts, out_type);
-  p.loose = direct && !even;
-  return ph_launch_w8_product(p, p.loose ? any : w.choice, out_type, (hipStream_t)stream);
+  p.loose = way.loose;
+  return ph_launch_w8_product(p, way.choice, out_type, (hipStream_t)stream);
 }
 
 int ph_w8_linear(int device, void* stream, const void* x, int x_type, const ph_rows* rows, const ph_w8_layer* layer, void* out,

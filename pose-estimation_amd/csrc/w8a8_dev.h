@@ -161,10 +161,10 @@ __device__ __forceinline__ void w8_finish4(const PhW8Params& p, const i32x4 a, u
   w8_store4<O>((O*)p.out + ph_row_off(p.outr, m) + n, w8_values_of(a, w8_channels(p, n), s, p.act), p.N - n);
 }
 
-// A wave's TM x TN fragments -> out, tokens m0 + .. (s: the scales of a lane's tokens), channels n0 + ...  In a fragment the 16 lanes side by side hold 16
-// tokens (rows of out) and 4 channels each: stored like that, every 8-byte piece is a request of its own (13 us for a
-// 256 x 256 tile of bf16).  So two fragments' tokens at a time go through the wave's own LDS piece and leave as whole
-// rows of its channels, 16 bytes a lane.
+// A wave's TM x TN fragments -> out, tokens m0 + .. (s: the scales of a lane's tokens), channels n0 + ...  In a fragment the
+// 16 lanes side by side hold 16 tokens (rows of out) and 4 channels each: stored like that, every 8-byte piece is a request of
+// its own (13 us for a 256 x 256 tile of bf16).  So two fragments' tokens at a time go through the wave's own LDS piece and
+// leave as whole rows of its channels, 16 bytes a lane.
 template <int TM, int TN, typename O>
 struct WaveOut {
   static constexpr int ROW = TN * 16 * (int)sizeof(O);

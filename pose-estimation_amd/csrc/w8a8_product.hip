@@ -171,7 +171,8 @@ static int launch_tile(const PhW8Params& p, int parts, hipStream_t st) {
 // along K in turn and their sums meet in LDS.
 //
 // T is int8_t, or the type of float rows that the block quantises itself, into LDS, while its first weights are on their
-// way: for one to a few tokens that costs less than a launch of its own before this one (see launch_few_float).
+// way: for few tokens that costs less than a launch of its own before this one (ph_w8_few_float).
+
 // up to 64 rows -> int8 rows of `pitch` bytes and their scales in LDS, all rows at once: 512 / (their number rounded up to a
 // power of two) lanes a row
 template <int W, typename T>
@@ -220,21 +221,14 @@ __device__ __forceinline__ void quantize_block(const FloatRows& f, unsigned M, i
   __syncthreads();
 }
 
-// 16 bytes of a row of K >= 16 that starts anywhere, nothing read behind its end: where fewer are left, its last 16 and a
-// shift (the same in every lane that has one; what moves in meets zero weights)
-__device__ __forceinline__ i32x4 load_loose(const int8_t* row, int k, int K) {
-  typedef i32x4 any __attribute__((aligned(1)));
-  const int over = k + 16 - K;
-  i32x4 v = *(const any*)(row + (over > 0 ? K - 16 : k));
-  const int b = 16 - (K & 15);   // of the piece that the row's end cuts
-  if (over > 0) {
-    if (b & 8) v = i32x4{v[2], v[3], 0, 0};
-    if (b & 4) v = i32x4{v[1], v[2], v[3], 0};
-    const int bs = b & 3;
+// A row's last 16 bytes -> those from k on (k + 16 - K = `over` > 0; the shift is the same in every lane that has one, and what
+// moves in meets zero weights)
+__device__ __forceinline__ i32x4 tail_16(i32x4 v, int K) {
+  const int b = 16 - (K & 15), bs = b & 3;
+  if (b & 8) v = i32x4{v[2], v[3], 0, 0};
+  if (b & 4) v = i32x4{v[1], v[2], v[3], 0};
 #pragma unroll
-    for (int i = 0; i < 4; i++)
-      v[i] = (int)__builtin_amdgcn_alignbyte(i < 3 ? (unsigned)v[i + 1] : 0u, (unsigned)v[i], bs);
-  }
+  for (int i = 0; i < 4; i++) v[i] = (int)__builtin_amdgcn_alignbyte(i < 3 ? (unsigned)v[i + 1] : 0u, (unsigned)v[i], bs);
   return v;
 }
 
@@ -250,8 +244,9 @@ __global__ __launch_bounds__(64 * W) void w8_few_kernel(const PhW8Params p, cons
   const int fr = lane & 15, fq = lane >> 4;
   const int nb = blockIdx.x;
   const unsigned m0 = blockIdx.z * (16 * TM);
-  const int kb0 = SPLIT ? (int)((int64_t)p.nkb * blockIdx.y / gridDim.y) : 0;
-  const int kb1 = SPLIT ? (int)((int64_t)p.nkb * (blockIdx.y + 1) / gridDim.y) : p.nkb;
+  const int nk = (p.K + 63) >> 6;   // (a fragment of zeros that the weights may end with is left out)
+  const int kb0 = SPLIT ? (int)((int64_t)nk * blockIdx.y / gridDim.y) : 0;
+  const int kb1 = SPLIT ? (int)((int64_t)nk * (blockIdx.y + 1) / gridDim.y) : nk;
   const int8_t* const wp = p.w + (int64_t)nb * p.nkb * 1024 + lane * 16;
   i32x4 wf[DEPTH];
   auto weights = [&](int kb) {
@@ -270,6 +265,8 @@ __global__ __launch_bounds__(64 * W) void w8_few_kernel(const PhW8Params p, cons
     xp[i] = FLOAT ? nullptr : p.q + ph_row_off(p.qr, m);
     xq[i] = (int)m * pitch;
   }
+  typedef i32x4 any __attribute__((aligned(1)));
+  const int last = p.loose ? p.K - 16 : p.K;   // where the last 16 bytes start: nothing is read behind a loose row's end
   i32x4 acc[TM];
 #pragma unroll
   for (int i = 0; i < TM; i++) acc[i] = i32x4{0, 0, 0, 0};
@@ -277,15 +274,25 @@ __global__ __launch_bounds__(64 * W) void w8_few_kernel(const PhW8Params p, cons
     i32x4 xf[DEPTH][TM], w[DEPTH];
 #pragma unroll
     for (int d = 0; d < DEPTH; d++) {
+      if (kb + d * W >= kb1) break;
       int k = (kb + d * W) * 64 + fq * 16;
       k = k < p.K ? k : 0;   // units behind the row's end meet zero weights
 #pragma unroll
       for (int i = 0; i < TM; i++) {
         if constexpr (FLOAT) xf[d][i] = *(const i32x4*)(s_q + xq[i] + k);
-        else if (p.loose) xf[d][i] = load_loose(xp[i], k, p.K);
-        else xf[d][i] = *(const i32x4*)(xp[i] + k);
+        else xf[d][i] = *(const any*)(xp[i] + min(k, last));
       }
       w[d] = wf[d];
+    }
+    if (!FLOAT && p.loose) {
+#pragma unroll
+      for (int d = 0; d < DEPTH; d++) {
+        if (kb + d * W >= kb1 || (kb + d * W + 1) * 64 <= p.K) continue;   // (only the last fragment of a row has an end inside)
+        const int k = (kb + d * W) * 64 + fq * 16;
+        if (k > last && k < p.K)
+#pragma unroll
+          for (int i = 0; i < TM; i++) xf[d][i] = tail_16(xf[d][i], p.K);
+      }
     }
     weights(kb + W * DEPTH);
 #pragma unroll
@@ -351,15 +358,16 @@ static const Kernel kernels[N_KERNELS] = {
     {256, 256, 1, 1.72f, 1.72f, 6.f}, {128, 128, 2, 0.64f, 0.50f, 3.5f}, {128, 128, 1, 0.56f, 0.56f, 3.5f},
     {128, 64, 3, 0.55f, 0.32f, 2.6f}, {64, 64, 3, 0.32f, 0.20f, 2.2f}};
 
+// the parts' sums to memory, back, and the launch that joins them
+static float join_us(int64_t M, int64_t n16, int parts) { return parts > 1 ? 3.3f + (float)M * n16 * 4e-6f * parts / 2.f : 0.f; }   // (2 TB/s)
+
 // Splitting K pays where there are far fewer blocks than CUs: the parts' sums (4 bytes each) are written, read and
 // joined by a second launch.
 PhW8Choice ph_w8_choose(int64_t M, int N, int nkb) {
   const int steps = nkb / 2;
   const int64_t n16 = (N + 15) / 16 * 16;
   const float wire = (float)n16 * nkb * 64 / 5.5e6f;   // the weights, once, from memory
-  auto join = [&](int parts) { return parts > 1 ? 3.3f + (float)M * n16 * 4e-6f * parts / 2.f : 0.f; };   // (2 TB/s)
-  PhW8Choice best = {K_64, 1};
-  float least = 1e30f;
+  PhW8Choice best = {K_64, 1, 1e30f};
   const int64_t small = (M + 63) / 64 * ((N + 63) / 64);   // blocks of the smallest tile: two rounds of them need no parts
   for (int parts = 1; parts <= 32 && parts <= steps; parts *= 2) {
     if (parts > 1 && (small >= 1024 || (float)M * n16 * parts > (float)(1 << 24))) break;
@@ -369,26 +377,40 @@ PhW8Choice ph_w8_choose(int64_t M, int N, int nkb) {
       const int64_t blocks = (M + c.bm - 1) / c.bm * ((N + c.bn - 1) / c.bn) * parts;
       const int64_t each = (blocks + 255) / 256, rounds = (each + c.fit - 1) / c.fit;
       const float run = (float)s * (each * c.full > rounds * c.alone ? each * c.full : rounds * c.alone);
-      const float t = (run > wire ? run : wire) + rounds * c.fixed + join(parts);
-      if (t < least) least = t, best = {k, parts};
+      const float t = (run > wire ? run : wire) + rounds * c.fixed + join_us(M, n16, parts);
+      if (t < best.us) best = {k, parts, t};
     }
     if (M <= 64) {   // a wave's step is one fragment of 64 k; blocks' loads share the memory's rate
       const int tm = (int)(M + 15) / 16;
       const int64_t blocks = n16 / 16 * parts, rounds = (blocks + 511) / 512;
       const float run = (s * 2 + 31) / 32 * rounds * (0.35f + 0.45f * tm), w = wire * (0.8f + 0.2f * tm);
-      const float t = 1.f + 0.5f * tm + (run > w ? run : w) + join(parts);
-      if (t < least) least = t, best = {K_FEW, parts};
+      const float t = 1.f + 0.5f * tm + (run > w ? run : w) + join_us(M, n16, parts);
+      if (t < best.us) best = {K_FEW, parts, t};
     }
   }
   return best;
 }
 
-// Rows of any alignment: the few-token kernel takes them as they are, also for more tokens as long as its blocks' reading
-// of all rows (from cache) costs less than a launch that lays them out anew: 267 x 546 -> 2611 XX us, else 8.4.
+// Rows of any alignment: the few-token kernel takes them as they are, 64 tokens to a block, as long as that costs less than a
+// launch that lays them out anew (3.4 us and 16-byte pieces at 2 TB/s) and a product of those.  A load of 16 rows' 64 bytes that
+// start anywhere takes a CU 0.07 us (a fragment of aligned rows hardly anything), so long rows go the other way.
+// us, direct | laid out anew:
+//   1613 x 55 -> 22 3.6 | 7.3, 500 x 301 -> 300 4.7 | 7.5, 5000 x 31 -> 100 5.3 | 7.3, 70 x 1001 -> 40 6.1 | 8.1
+//   37 x 2047 -> 1001 11.2 | 8.7, 70 x 2001 -> 40 in one part 10.8, in four 6.6 | 9.4, 64 x 4001 -> 2000 23 | 12.5
 PhW8Choice ph_w8_choose_loose(int64_t M, int K, int N) {
+  const int nkb = (K + 63) / 64;
   const PhW8Choice c = ph_w8_choose(M, N, (K + 127) / 128 * 2);
-  if (K < 16 || (M <= 64 && c.kernel != K_FEW) || (M > 64 && (double)M * K * ((N + 15) / 16) > 3e6)) return {-1, 1};
-  return M <= 64 ? c : PhW8Choice{K_FEW, 1};
+  PhW8Choice best = {-1, 1, c.us + 3.4f + (float)M * K * 1e-6f};
+  if (K < 16) return best;
+  const int64_t n16 = (N + 15) / 16 * 16;
+  const int tm = M > 48 ? 4 : (int)(M + 15) / 16;
+  for (int parts = 1; parts <= 8 && parts <= (nkb + 1) / 2; parts *= 2) {
+    if (parts > 1 && (float)M * n16 * parts > (float)(1 << 22)) break;
+    const int64_t rounds = ((M + 63) / 64 * (n16 / 16) * parts + 255) / 256;
+    const float t = 2.5f + (float)rounds * (0.7f + 0.07f * tm * ((nkb + parts - 1) / parts)) + join_us(M, n16, parts);
+    if (t < best.us) best = {K_FEW, parts, t};
+  }
+  return best;
 }
 
 int64_t ph_w8_parts_bytes(const PhW8Choice& c, int64_t M, int N) {

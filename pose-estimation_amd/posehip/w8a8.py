@@ -8,7 +8,7 @@ network runs in 8 bits; ``cv2.dnn``'s quantised networks do the same per channel
     y = linear(x, layer)                                            # x [..,K] float -> [..,N]
     q, s = quantize_rows(x)                                         # once, for several layers that read x
     y1, y2 = matmul(q, s, layer1), matmul(q, s, layer2)
-    y = feed_forward(x, layer1, layer2)                             # two layers, nothing between them in memory's way
+    y = feed_forward(x, layer1, layer2)                             # two layers, in one kernel where they fit
 
     s[m]   = max(f32(max_k |x[m,k]| / 127), 2^-126)      q[m,k] = round_half_even(x[m,k] / s[m])   (exact quotient)
     y[m,n] = act((f32(sum_k q[m,k] w[n,k]) * ws[n]) * s[m] + bias[n])
@@ -16,7 +16,8 @@ network runs in 8 bits; ``cv2.dnn``'s quantised networks do the same per channel
 The sum is an exact 32-bit integer (K <= 131071), each later operation is rounded to f32, the result once to its type;
 so ``linear(x, l)`` is ``matmul(*quantize_rows(x), l)`` and ``feed_forward(x, a, b)`` is
 ``linear(linear(x, a, dtype=torch.float32), b)``, both bit for bit, whatever the sizes.  A row with a NaN or an infinity
-gives NaN outputs and touches no other row.  There are no gradients: tensors that ask for one are refused.
+gives NaN outputs and touches no other row.  There are no gradients: inputs and outputs that ask
+for one are refused (a Layer takes a parameter's values as they are).
 
 Tensors are CUDA tensors of f32 / f16 / bf16 with the values of a row consecutive (last stride 1) and any other strides;
 leading dimensions that do not merge into three are refused.  Work is put on torch's current stream of the tensors'

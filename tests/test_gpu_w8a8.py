@@ -263,7 +263,8 @@ def test_feed_forward_borders(w8, M, K, H, N):
 
 
 @pytest.mark.parametrize("M,K,N", [(1, 15, 20), (1, 16, 20), (5, 17, 33), (64, 31, 100), (65, 33, 100), (64, 4099, 100), (200, 47, 70), (3, 40001, 5),
-                                   (700, 1001, 90), (64, 64, 64)])
+                                   (700, 1001, 90), (64, 64, 64), (70, 4001, 40), (200, 2001, 33), (64, 1001, 40), (48, 31, 3000),
+                                   (3000, 55, 100), (300, 16, 20), (33, 1040, 50)])
 def test_matmul_of_rows_that_start_anywhere(w8, M, K, N):
     """Nothing behind the last row's end is read: the storage ends there, and what stands before and between is noise."""
     rng = np.random.default_rng(K + M)
@@ -430,6 +431,17 @@ def test_first_calls_inside_a_capture(w8):
         e = (w8.feed_forward(dx, l1, l2), w8.linear(dx, l1), w8.linear(dv, l3, dtype=torch.float16))
         torch.cuda.synchronize()
         assert all(torch.equal(p, r) for p, r in zip(o, e))
+
+
+def test_a_device_that_is_not_there(w8):
+    """A call for one is refused, and nothing of it is left for the next call."""
+    from posehip import _ffi
+    x = torch.ones(4, 64, device="cuda")
+    rows, _ = w8._rows(x.shape, x.stride())
+    for device in (torch.cuda.device_count() + 3, -1):
+        assert _ffi.lib().ph_w8_quantize_rows(device, None, x.data_ptr(), _ffi.PH_F32, rows, 64, x.data_ptr(), 64, x.data_ptr()) == -1
+        q, s = w8.quantize_rows(x)
+        assert q.min() == 127 and s.max() > 0
 
 
 def test_more_rows_than_a_launch_holds(w8):

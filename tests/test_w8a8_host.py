@@ -69,7 +69,7 @@ def test_c_refusals():
     assert lib.ph_w8_workspace(0, -1, 4, 0, 4) == -1 and lib.ph_w8_workspace(1, 4, 0, 0, 4) == -1
     q = lambda **k: lib.ph_w8_quantize_rows(0, None, k.get("x", 4096), k.get("t", 0), k.get("rows", rows()), k.get("k", 64),   # noqa: E731
                                             k.get("q", 4096), k.get("pitch", 64), k.get("s", 4096))
-    assert q(t=3) == -1 and q(t=-1) == -1 and q(k=0) == -1 and q(pitch=48) == -1 and q(pitch=72) == -1 and q(q=4104) == -1
+    assert q(t=3) == -1 and q(t=-1) == -1 and q(k=0) == -1 and q(k=(1 << 30) + 1, pitch=1 << 31) == -1 and q(pitch=48) == -1 and q(pitch=72) == -1 and q(q=4104) == -1
     assert q(x=None) == -1 and q(s=None) == -1 and q(q=None) == -1
     assert q(rows=rows((1, -1, 4))) == -1 and q(rows=rows((1, 1 << 16, 1 << 15))) == -1 and q(rows=rows((1 << 31, 1, 1))) == -1
     assert q(rows=rows((1, 0, 4)), x=None) == 0 and q(rows=rows((0, 1 << 40, 1 << 40))) == 0
@@ -81,8 +81,9 @@ def test_c_refusals():
     odd = layer()
     odd.scale = 4104
     assert m(layer=odd) == -1
-    r = rows((1, 1, 100000))
-    assert m(q=4097, rows=r) == -3 and m(rows=rows((1, 1, 100000), (0, 0, 65))) == -3 and m(q=4097, rows=r, ws=4096 + 16, nws=1 << 20) == -3
+    r, big = rows((1, 1, 100000), (0, 0, 4096)), layer(n=640, k=4000)
+    assert m(q=4097, rows=r, layer=big) == -3 and m(rows=rows((1, 1, 100000), (0, 0, 4097)), layer=big) == -3
+    assert m(q=4097, rows=r, layer=big, ws=4096 + 16, nws=1 << 40) == -3
     assert b"workspace" in lib.ph_last_error()
     li = lambda **k: lib.ph_w8_linear(0, None, k.get("x", 4096), k.get("t", 0), k.get("rows", rows((1, 1, 100))), layer(k=4000), 4096, k.get("ot", 0),   # noqa: E731
                                       st, k.get("ws", 4096), k.get("nws", 1 << 20))
