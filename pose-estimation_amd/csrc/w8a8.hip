@@ -51,12 +51,12 @@ __global__ __launch_bounds__(G <= 64 ? 256 : G) void quantize_rows_kernel(const 
 #pragma unroll
   for (int c = 0; c < CH; c++) {
     const int k = c * STEP + lane * 8;
-    if (k < K) *(uint64_t*)(qrow + k) = v[c].quantize(r) >> Eight<T>::shift(k, K);
+    if (k < K) *(uint64_t*)(qrow + k) = v[c].template quantize<true>(r) >> Eight<T>::shift(k, K);
   }
   for (int k = CH * STEP + lane * 8; k < K; k += STEP) {
     Eight<T> t;
     t.load(row, k, K);
-    *(uint64_t*)(qrow + k) = t.quantize(r) >> Eight<T>::shift(k, K);
+    *(uint64_t*)(qrow + k) = t.template quantize<true>(r) >> Eight<T>::shift(k, K);
   }
 }
 

@@ -233,7 +233,7 @@ __global__ __launch_bounds__(512, 4) void w8_pair_kernel(const PhW8Pair p) {
     unsigned o[4];
 #pragma unroll
     for (int e = 0; e < 16; e++) v[e] = __uint_as_float((unsigned)acc[e >> 2][i][e & 3]);
-    quantize_n(v, r, o);
+    quantize_n<false>(v, r, o);
 #pragma unroll
     for (int j = 0; j < 4; j++) *(unsigned*)(q + (i * 16 + fr) * PITCH + (wave * 4 + j) * 16 + fq * 4) = o[j];
     __builtin_amdgcn_sched_barrier(0);

@@ -101,6 +101,25 @@ def test_quantize_many_values_near_borders(w8):
     assert np.array_equal(sc.cpu().numpy(), ws) and np.array_equal(q.cpu().numpy(), wq)
 
 
+@pytest.mark.parametrize("e", [-126, -125, -124, -100, -30, -1, 0, 1, 60, 120])
+@pytest.mark.parametrize("step", [-1, 0, 1])
+def test_quantize_next_to_every_border(w8, e, step):
+    """The float next to each border k + 1/2, and those beside it, down to scales whose half is no float any more."""
+    rng = np.random.default_rng(e + 200)
+    M = 512
+    amax = (127 * (1 + rng.integers(0, 1 << 22, M) * 2.0 ** -22) * 2.0 ** e).astype(np.float32)
+    s = np.maximum((amax.astype(np.float64) / 127).astype(np.float32), np.float32(2.0 ** -126))
+    k = np.arange(-127, 127)[None] + 0.5
+    x = (k * s[:, None].astype(np.float64)).astype(np.float32)
+    if step:
+        x = np.nextafter(x, np.float32(step * np.inf), dtype=np.float32)
+    x = np.where(np.abs(x) < amax[:, None], x, amax[:, None])
+    x[:, 100] = amax
+    q, sc = w8.quantize_rows(torch.from_numpy(x).cuda())
+    wq, ws = ref.quantize_rows(x)
+    assert np.array_equal(sc.cpu().numpy(), ws) and np.array_equal(q.cpu().numpy(), wq)
+
+
 @pytest.mark.parametrize("t", ["f32", "bf16"])
 def test_quantize_strided_rows(w8, t):
     rng = np.random.default_rng(3)
