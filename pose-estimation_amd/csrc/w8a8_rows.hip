@@ -177,18 +177,15 @@ __global__ __launch_bounds__(512, 4) void w8_pair_kernel(const PhW8Pair p) {
   i32x4 wa[4];
 #pragma unroll
   for (int j = 0; j < 4; j++) wp[j] = p.w1 + (int64_t)min(wave * 4 + j, p.nnb1 - 1) * p.nkb1 * 1024 + lane * 16;
-  rows_to_lds<TF, T>(p.x, p.xr, p.M, p.K, m0, q, s1, tid, [&] {   // (while the rows are on their way)
-    for (int n = tid; n < PAIR_MAX; n += 512) {   // (channels that do not exist: zeros)
-      const bool is = n < p.nnb1 * 16;
-      par[n] = is ? p.ws1[n] : 0.f;
-      par[PAIR_MAX + n] = is && p.bias1 ? p.bias1[n] : 0.f;
-      par[2 * PAIR_MAX + n] = is && p.slope1 ? p.slope1[n] : 0.f;
-    }
-    for (int f = wave; f < p.nnb2 * p.nkb2; f += 8)
-      __builtin_amdgcn_global_load_lds((glb_void*)(p.w2 + f * 1024 + lane * 16), (lds_void*)(w2 + f * 1024), 16, 0, 0);
-  });
+  // (from cache, so here before the rows, which loads that return in order would hold up otherwise)
+  for (int f = wave; f < p.nnb2 * p.nkb2; f += 8)
+    __builtin_amdgcn_global_load_lds((glb_void*)(p.w2 + f * 1024 + lane * 16), (lds_void*)(w2 + f * 1024), 16, 0, 0);
+  const bool is = tid < p.nnb1 * 16;   // (channels that do not exist: zeros)
+  const float par0 = is ? p.ws1[tid] : 0.f, par1 = is && p.bias1 ? p.bias1[tid] : 0.f, par2 = is && p.slope1 ? p.slope1[tid] : 0.f;
 #pragma unroll
   for (int j = 0; j < 4; j++) wa[j] = *(const i32x4*)wp[j];
+  rows_to_lds<TF, T>(p.x, p.xr, p.M, p.K, m0, q, s1, tid, [&] {});
+  par[tid] = par0, par[PAIR_MAX + tid] = par1, par[2 * PAIR_MAX + tid] = par2;
   __syncthreads();
   const char* const xq = q + fr * PITCH + fq * 16;
   i32x4 acc[4][TF];
@@ -250,13 +247,18 @@ __global__ __launch_bounds__(512, 4) void w8_pair_kernel(const PhW8Pair p) {
   const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
   const Channels c2 = {*(const f32x4*)(p.ws2 + at), p.bias2 ? *(const f32x4*)(p.bias2 + at) : zero, p.slope2 ? *(const f32x4*)(p.slope2 + at) : zero};
   const char* const wq = w2 + min(nb2, p.nnb2 - 1) * p.nkb2 * 1024 + lane * 16;
-  for (int kb = 0; kb < p.nkb2; kb++) {
-    const i32x4 w = *(const i32x4*)(wq + kb * 1024);
+  for (int kb = 0; kb < p.nkb2; kb += 2) {   // (an even number)
+    i32x4 w[2], xf[2][U];
 #pragma unroll
-    for (int u = 0; u < U; u++) {
-      const int i = t0 + u * dt;
-      if (i < TF) z[u] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w, *(const i32x4*)(xq + i * 16 * PITCH + kb * 64), z[u], 0, 0, 0);
+    for (int b = 0; b < 2; b++) {
+      w[b] = *(const i32x4*)(wq + (kb + b) * 1024);
+#pragma unroll
+      for (int u = 0; u < U; u++) xf[b][u] = *(const i32x4*)(xq + min(t0 + u * dt, TF - 1) * 16 * PITCH + (kb + b) * 64);
     }
+#pragma unroll
+    for (int b = 0; b < 2; b++)
+#pragma unroll
+      for (int u = 0; u < U; u++) z[u] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[b], xf[b][u], z[u], 0, 0, 0);
   }
 #pragma unroll
   for (int u = 0; u < U; u++) {
