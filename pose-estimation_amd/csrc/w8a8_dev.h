@@ -34,21 +34,23 @@ __device__ __forceinline__ float max_group(float m) {
 }
 
 struct RowScale {
-  float s, inv, half;   // scale, 1 / scale, scale / 2
+  float s, inv, half;   // scale, 1 / scale to 2^-23 of it, scale / 2
   bool finite;
 };
 __device__ __forceinline__ RowScale row_scale(float amax) {
   RowScale r;
   r.finite = amax < __builtin_inff();
-  r.s = r.finite ? fmaxf(amax / 127.f, 0x1p-126f) : 1.f;
-  r.inv = 1.f / r.s;
+  // amax / 127, rounded as a division rounds it (compared for every f32)
+  const float y = amax * (1.f / 127.f);
+  r.s = r.finite ? fmaxf(__builtin_fmaf(__builtin_fmaf(-127.f, y, amax), 1.f / 127.f, y), 0x1p-126f) : 1.f;
+  r.inv = __builtin_amdgcn_rcpf(r.s);
   r.half = 0.5f * r.s;
   return r;
 }
 __device__ __forceinline__ float scale_out(const RowScale& r) { return r.finite ? r.s : __builtin_nanf(""); }
 
 // round_half_even(x / s), N values to N bytes; ZERO: zeros for a row that is not finite (else anything).  Adding 1.5 * 2^23
-// rounds to a whole number, which then stands in the low bits of the sum.  x * (1/s) is within 127 * 2^-23 of the quotient, so
+// rounds to a whole number, which then stands in the low bits of the sum.  x * (1/s) is within 127 * 2^-22 of the quotient, so
 // that number is the wanted one or its neighbour; the remainder x - q s is exact in one fused operation and tells which.
 // Where no remainder reaches half a step, as almost always, all stand.  (One rounding that leaves the fraction in the sum's
 // low bits takes an operation less, but shifts and integer minima run at half the rate of fma and add: 28 -> 30 us.)
@@ -79,6 +81,13 @@ __device__ __forceinline__ void quantize_n(const float (&x)[N], const RowScale& 
   }
 }
 
+template <bool ZERO = false>
+__device__ __forceinline__ uint64_t quantize_8(const float (&x)[8], const RowScale& r) {
+  unsigned o[2];
+  quantize_n<ZERO>(x, r, o);
+  return (uint64_t)o[1] << 32 | o[0];
+}
+
 // Eight values of a row from k on; rows start at any multiple of their element.  Where fewer are left, the row's last
 // eight: a value seen twice does not change a maximum, and the bytes move to their place by `shift` bits.
 template <typename T>
@@ -100,14 +109,15 @@ struct Eight {
     for (int i = 0; i < 8; i++) m = max_abs(m, (float)v[i]);
     return m;
   }
+  __device__ __forceinline__ void to_floats(float (&x)[8]) const {
+#pragma unroll
+    for (int i = 0; i < 8; i++) x[i] = (float)v[i];
+  }
   template <bool ZERO = false>
   __device__ __forceinline__ uint64_t quantize(const RowScale& r) const {
     float x[8];
-    unsigned o[2];
-#pragma unroll
-    for (int i = 0; i < 8; i++) x[i] = (float)v[i];
-    quantize_n<ZERO>(x, r, o);
-    return (uint64_t)o[1] << 32 | o[0];
+    to_floats(x);
+    return quantize_8<ZERO>(x, r);
   }
 };
 

@@ -5,31 +5,40 @@ constexpr int PITCH = PAIR_MAX + 16;   // of an 8-bit row in LDS: 16 rows' units
 
 // rows m0 .. of 8 <= K <= 512 values -> 8 bits and scales in LDS; 16 lanes a row, 32 rows at a time, 4 chunks of 128 values
 template <int TF, typename T, typename Between>
-__device__ __forceinline__ void rows_to_lds(const void* x, const PhRowMap& xr, unsigned M, int K, unsigned m0, char* q, float* s,
+__device__ __forceinline__ void rows_to_lds(const void* rows, const PhRowMap& xr, unsigned M, int K, unsigned m0, char* q, float* s,
                                             int tid, Between between) {
   constexpr int RP = TF / 2, CH = 4;
   Eight<T> raw[RP][CH];
 #pragma unroll
   for (int r = 0; r < RP; r++) {
-    const T* row = (const T*)x + ph_row_off(xr, min(m0 + r * 32 + (tid >> 4), M - 1));
+    const T* row = (const T*)rows + ph_row_off(xr, min(m0 + r * 32 + (tid >> 4), M - 1));
 #pragma unroll
     for (int c = 0; c < CH; c++)
       if (c * 128 < K) raw[r][c].load_long(row, c * 128 + (tid & 15) * 8, K);
   }
   between();
+  float x[RP][CH][8];
+  RowScale sc[RP];
 #pragma unroll
   for (int r = 0; r < RP; r++) {
     float am = 0.f;
 #pragma unroll
     for (int c = 0; c < CH; c++)
-      if (c * 128 < K) am = raw[r][c].max_with(am);
-    const RowScale sc = row_scale(max_group<16>(am));
+      if (c * 128 < K) {
+        raw[r][c].to_floats(x[r][c]);
+#pragma unroll
+        for (int i = 0; i < 8; i++) am = max_abs(am, x[r][c][i]);
+      }
+    sc[r] = row_scale(max_group<16>(am));
+  }
+#pragma unroll
+  for (int r = 0; r < RP; r++) {
     const int t = r * 32 + (tid >> 4);
-    if ((tid & 15) == 0) s[t] = scale_out(sc);
+    if ((tid & 15) == 0) s[t] = scale_out(sc[r]);
 #pragma unroll
     for (int c = 0; c < CH; c++) {
       const int k = c * 128 + (tid & 15) * 8;
-      if (k < K) *(uint64_t*)(q + t * PITCH + k) = raw[r][c].quantize(sc) >> Eight<T>::shift(k, K);
+      if (k < K) *(uint64_t*)(q + t * PITCH + k) = quantize_8(x[r][c], sc[r]) >> Eight<T>::shift(k, K);
     }
   }
 }
@@ -160,6 +169,8 @@ int ph_launch_w8_rows(const PhW8Params& p, const FloatRows& f, int x_type, int o
 // (weights straight from cache, each fragment read by one wave and used for TF products); inner values and their maxima;
 // inner rows in 8 bits into the same LDS; second product, its weights in LDS for good.  Two blocks share a CU, so that one's
 // rounding (12 vector operations per inner value) runs under the other's products.
+constexpr int AHEAD = 512;   // blocks that run at a time: two on each of 256 CUs
+
 template <int TF, int ACT, typename T>
 __global__ __launch_bounds__(512, 4) void w8_pair_kernel(const PhW8Pair p) {
   constexpr int BT = 16 * TF;
@@ -169,7 +180,8 @@ __global__ __launch_bounds__(512, 4) void w8_pair_kernel(const PhW8Pair p) {
   float* const s2 = s1 + BT;
   float* const red = s2 + BT;                         // [8][BT]
   float* const par = red + 8 * BT;                    // scale, bias, slope of the inner channels [3][PAIR_MAX]
-  char* const w2 = (char*)(par + 3 * PAIR_MAX);
+  float* const par2 = par + 3 * PAIR_MAX;             // of the outputs [3][64]
+  char* const w2 = (char*)(par2 + 3 * 64);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int fr = lane & 15, fq = lane >> 4;
   const unsigned m0 = blockIdx.x * BT;
@@ -181,15 +193,30 @@ __global__ __launch_bounds__(512, 4) void w8_pair_kernel(const PhW8Pair p) {
   for (int f = wave; f < p.nnb2 * p.nkb2; f += 8)
     __builtin_amdgcn_global_load_lds((glb_void*)(p.w2 + f * 1024 + lane * 16), (lds_void*)(w2 + f * 1024), 16, 0, 0);
   const bool is = tid < p.nnb1 * 16;   // (channels that do not exist: zeros)
-  const float par0 = is ? p.ws1[tid] : 0.f, par1 = is && p.bias1 ? p.bias1[tid] : 0.f, par2 = is && p.slope1 ? p.slope1[tid] : 0.f;
+  float out_par = 0.f;
+  if (tid < 3 * 64 && (tid & 63) < p.nnb2 * 16) {
+    const float* const from = tid < 64 ? p.ws2 : tid < 128 ? p.bias2 : p.slope2;
+    if (from) out_par = from[tid & 63];
+  }
+  const float par0_ = is ? p.ws1[tid] : 0.f, par1_ = is && p.bias1 ? p.bias1[tid] : 0.f, par2_ = is && p.slope1 ? p.slope1[tid] : 0.f;
 #pragma unroll
   for (int j = 0; j < 4; j++) wa[j] = *(const i32x4*)wp[j];
   rows_to_lds<TF, T>(p.x, p.xr, p.M, p.K, m0, q, s1, tid, [&] {});
-  par[tid] = par0, par[PAIR_MAX + tid] = par1, par[2 * PAIR_MAX + tid] = par2;
+  par[tid] = par0_, par[PAIR_MAX + tid] = par1_, par[2 * PAIR_MAX + tid] = par2_;
+  if (tid < 3 * 64) par2[tid] = out_par;
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the second layer's weights are in LDS (as the rows, requested after them)
   __syncthreads();
   const char* const xq = q + fr * PITCH + fq * 16;
   i32x4 acc[4][TF];
   rows_product<TF>(xq, wp, wa, p.nkb1, acc);
+  // A line of each 128 bytes of the rows that the block after the next on this CU will read: its loads find them in L2.
+  T ahead = T(0.f);
+  if (TF == 4) {
+    const int64_t m = (int64_t)m0 + AHEAD * BT + (tid >> 3);
+    const int k = (tid & 7) * (128 / (int)sizeof(T));
+    ahead = ((const T*)p.x)[ph_row_off(p.xr, m < p.M ? (unsigned)m : p.M - 1) + min(k, p.K - 1)];
+  }
+  __builtin_amdgcn_sched_barrier(0);
   // inner values, in place of their sums, and each row's maximum
   float am[TF], sc[TF];
 #pragma unroll
@@ -217,7 +244,6 @@ __global__ __launch_bounds__(512, 4) void w8_pair_kernel(const PhW8Pair p) {
     am[i] = max_32(max_16(am[i]));
     if (fq == 0) red[wave * BT + i * 16 + fr] = am[i];
   }
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the second layer's weights are in LDS
   __syncthreads();   // the first product is done everywhere: q is free
 #pragma unroll
   for (int i = 0; i < TF; i++) {
@@ -243,9 +269,7 @@ __global__ __launch_bounds__(512, 4) void w8_pair_kernel(const PhW8Pair p) {
 #pragma unroll
   for (int u = 0; u < U; u++) z[u] = i32x4{0, 0, 0, 0};
   const int n = nb2 * 16 + fq * 4;
-  const int at = min(n, p.nnb2 * 16 - 4);
-  const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-  const Channels c2 = {*(const f32x4*)(p.ws2 + at), p.bias2 ? *(const f32x4*)(p.bias2 + at) : zero, p.slope2 ? *(const f32x4*)(p.slope2 + at) : zero};
+  const Channels c2 = {*(const f32x4*)(par2 + n), *(const f32x4*)(par2 + 64 + n), *(const f32x4*)(par2 + 128 + n)};
   const char* const wq = w2 + min(nb2, p.nnb2 - 1) * p.nkb2 * 1024 + lane * 16;
   for (int kb = 0; kb < p.nkb2; kb += 2) {   // (an even number)
     i32x4 w[2], xf[2][U];
@@ -282,6 +306,7 @@ __global__ __launch_bounds__(512, 4) void w8_pair_kernel(const PhW8Pair p) {
       }
     }
   }
+  if (TF == 4) asm volatile("" ::"v"(ahead));
 }
 
 bool ph_w8_pair_fits(int K, int H, int N) { return K >= 8 && K <= PAIR_MAX && H <= PAIR_MAX && N <= 64; }
@@ -289,7 +314,7 @@ bool ph_w8_pair_fits(int K, int H, int N) { return K >= 8 && K <= PAIR_MAX && H 
 template <int TF, int ACT, typename T>
 static int launch_pair_f(const PhW8Pair& p, hipStream_t st) {
   constexpr int BT = 16 * TF;
-  const int lds = BT * PITCH + 10 * BT * 4 + 12 * PAIR_MAX + p.nnb2 * p.nkb2 * 1024;   // <= 74 KB: two blocks a CU
+  const int lds = BT * PITCH + 10 * BT * 4 + 12 * PAIR_MAX + 12 * 64 + p.nnb2 * p.nkb2 * 1024;   // <= 74 KB: two blocks a CU
   static int granted[PH_MAX_DEVICES];
   if (lds > 64 * 1024 && ph_ensure_lds((const void*)w8_pair_kernel<TF, ACT, T>, lds, granted)) return -1;
   if (ph_w8_launchable((p.M - 1) / BT + 1, 512)) return -1;
