@@ -3,7 +3,7 @@
 
 constexpr int PITCH = PAIR_MAX + 16;   // of an 8-bit row in LDS: 16 rows' units lie in different banks
 
-// rows m0 .. of 8 <= K <= 512 values -> 8 bits and scales in LDS; 16 lanes a row, 32 rows at a time, 4 chunks of 128 values
+// rows m0 .. of 8 <= K <= 512 values -> 8 bits and scales in LDS; 16 lanes a row, 32 rows at a time, 4 chunks of 128 values.
 template <int TF, typename T, typename Between>
 __device__ __forceinline__ void rows_to_lds(const void* rows, const PhRowMap& xr, unsigned M, int K, unsigned m0, char* q, float* s,
                                             int tid, Between between) {
@@ -132,9 +132,9 @@ static int launch_rows_f(const PhW8Params& p, const FloatRows& f, hipStream_t st
   return 0;
 }
 // us for bf16 -> bf16, beside quantisation and product in two launches:
-//   32 tokens x 256 channels: 3772 x 288 -> 256 6.5 (two launches 7.9), 3772 x 512 -> 26 7.4 (8.6), 1000 x 200 -> 4000 7.6 (8.7)
-//   64 x 512: 120704 x 384 -> 512 65 (82), 30176 x 384 -> 1024 34 (39), 30176 x 512 -> 2048 69 (71)
-//   64 x 256: 120704 x 288 -> 256 40 (48);  64 x 128: 120704 x 512 -> 52 43 (52), 120704 x 384 -> 128 39 (48)
+//   32 tokens x 256 channels: 3772 x 288 -> 256 6.4 (two launches 7.8), 3772 x 512 -> 26 7.1 (8.3), 1000 x 200 -> 4000 7.3 (8.4)
+//   64 x 512: 120704 x 384 -> 512 57 (75), 30176 x 384 -> 1024 28 (38), 30176 x 512 -> 2048 63 (69)
+//   64 x 256: 120704 x 288 -> 256 40 (47);  64 x 128: 120704 x 512 -> 52 47 (50), 120704 x 384 -> 128 40 (47)
 bool ph_w8_rows_fit(int64_t M, int K, int N) { return K >= 8 && K <= PAIR_MAX && N <= (M <= 8192 ? 4096 : 2048); }
 
 template <typename T, typename O>
@@ -169,6 +169,9 @@ int ph_launch_w8_rows(const PhW8Params& p, const FloatRows& f, int x_type, int o
 // (weights straight from cache, each fragment read by one wave and used for TF products); inner values and their maxima;
 // inner rows in 8 bits into the same LDS; second product, its weights in LDS for good.  Two blocks share a CU, so that one's
 // rounding (12 vector operations per inner value) runs under the other's products.
+// 120704 x 384 -> 512 -> 52 bf16: 68 us (its bytes 22, its products 22).  Of a block's 15.6 us: rows 1.6, their rounding 3.0,
+// waiting for each other 1.3, first product 2.9, inner values 2.2, their rounding 2.3, second product 1.3, output 1.0: the vector
+// units bound it, busy for 40 us of the 68 (fma, add, mul take 2 cycles a wave; conversions, maxima, compares, shifts 4).
 constexpr int AHEAD = 512;   // blocks that run at a time: two on each of 256 CUs
 
 template <int TF, int ACT, typename T>
@@ -209,7 +212,8 @@ __global__ __launch_bounds__(512, 4) void w8_pair_kernel(const PhW8Pair p) {
   const char* const xq = q + fr * PITCH + fq * 16;
   i32x4 acc[4][TF];
   rows_product<TF>(xq, wp, wa, p.nkb1, acc);
-  // A line of each 128 bytes of the rows that the block after the next on this CU will read: its loads find them in L2.
+  // A line of each 128 bytes of the rows that the block after the next on this CU will read: its loads find them in L2
+  // (2.4 -> 1.6 us a block).
   T ahead = T(0.f);
   if (TF == 4) {
     const int64_t m = (int64_t)m0 + AHEAD * BT + (tid >> 3);
@@ -261,48 +265,56 @@ __global__ __launch_bounds__(512, 4) void w8_pair_kernel(const PhW8Pair p) {
     for (int j = 0; j < 4; j++) *(unsigned*)(q + (i * 16 + fr) * PITCH + (wave * 4 + j) * 16 + fq * 4) = o[j];
     __builtin_amdgcn_sched_barrier(0);
   }
+  // (read here, under the rounding: one after the other behind the last product they take 0.5 us)
+  PhW8Out o = p.out[0];
+  const int act2 = p.act2, n_out = p.n_out, nnb2 = p.nnb2, nkb2 = p.nkb2;
+  asm volatile("" ::"s"(o.p), "s"(o.step), "s"(o.type), "s"(o.r.flat), "s"(o.r.s2), "s"(act2), "s"(n_out), "s"(nnb2), "s"(nkb2));
   __syncthreads();
   // second product: a wave has one fragment of channels and every dt-th fragment of tokens
-  const int div = p.nnb2 > 2 ? 4 : p.nnb2, nb2 = wave % div, t0 = wave / div, dt = 8 / div;
+  const int div = nnb2 > 2 ? 4 : nnb2, nb2 = wave % div, t0 = wave / div, dt = 8 / div;
   constexpr int U = TF / 2;
   i32x4 z[U];
 #pragma unroll
   for (int u = 0; u < U; u++) z[u] = i32x4{0, 0, 0, 0};
   const int n = nb2 * 16 + fq * 4;
   const Channels c2 = {*(const f32x4*)(par2 + n), *(const f32x4*)(par2 + 64 + n), *(const f32x4*)(par2 + 128 + n)};
-  const char* const wq = w2 + min(nb2, p.nnb2 - 1) * p.nkb2 * 1024 + lane * 16;
-  for (int kb = 0; kb < p.nkb2; kb += 2) {   // (an even number)
-    i32x4 w[2], xf[2][U];
+  const char* const wq = w2 + min(nb2, nnb2 - 1) * nkb2 * 1024 + lane * 16;
+  for (int kb = 0; kb < nkb2; kb += 4) {
+    i32x4 w[4], xf[4][U];
 #pragma unroll
-    for (int b = 0; b < 2; b++) {
-      w[b] = *(const i32x4*)(wq + (kb + b) * 1024);
+    for (int b = 0; b < 4; b++) {
+      const int at = min(kb + b, nkb2 - 1);
+      w[b] = *(const i32x4*)(wq + at * 1024);
 #pragma unroll
-      for (int u = 0; u < U; u++) xf[b][u] = *(const i32x4*)(xq + min(t0 + u * dt, TF - 1) * 16 * PITCH + (kb + b) * 64);
+      for (int u = 0; u < U; u++) xf[b][u] = *(const i32x4*)(xq + min(t0 + u * dt, TF - 1) * 16 * PITCH + at * 64);
     }
 #pragma unroll
-    for (int b = 0; b < 2; b++)
+    for (int b = 0; b < 4; b++)
+      if (kb + b < nkb2)
 #pragma unroll
-      for (int u = 0; u < U; u++) z[u] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[b], xf[b][u], z[u], 0, 0, 0);
+        for (int u = 0; u < U; u++) z[u] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[b], xf[b][u], z[u], 0, 0, 0);
   }
+  f32x4 v[U];
 #pragma unroll
-  for (int u = 0; u < U; u++) {
-    const int i = t0 + u * dt;
-    const unsigned m = m0 + i * 16 + fr;
-    if (i >= TF || m >= p.M || n >= p.N || nb2 >= p.nnb2) continue;
-    const f32x4 v = w8_values_of(z[u], c2, s2[i * 16 + fr], p.act2);
-    for (int d = 0; d < p.n_out; d++) {
-      const PhW8Out& o = p.out[d];
+  for (int u = 0; u < U; u++) v[u] = w8_values_of(z[u], c2, s2[min(t0 + u * dt, TF - 1) * 16 + fr], act2);
+  for (int d = 0; d < n_out; d++) {
+    if (d) o = p.out[d];
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      const int i = t0 + u * dt;
+      const unsigned m = m0 + i * 16 + fr;
+      if (i >= TF || m >= p.M || n >= p.N || nb2 >= nnb2) continue;
       const int64_t off = ph_row_off(o.r, m) + n * o.step;
       if (o.step != 1) {   // planes of f32
 #pragma unroll
         for (int e = 0; e < 4; e++)
-          if (n + e < p.N) ((float*)o.p)[off + e * o.step] = v[e];
+          if (n + e < p.N) ((float*)o.p)[off + e * o.step] = v[u][e];
       } else if (o.type == PH_F32) {
-        w8_store4<float>((float*)o.p + off, v, p.N - n);
+        w8_store4<float>((float*)o.p + off, v[u], p.N - n);
       } else if (o.type == PH_F16) {
-        w8_store4<_Float16>((_Float16*)o.p + off, v, p.N - n);
+        w8_store4<_Float16>((_Float16*)o.p + off, v[u], p.N - n);
       } else {
-        w8_store4<bf16>((bf16*)o.p + off, v, p.N - n);
+        w8_store4<bf16>((bf16*)o.p + off, v[u], p.N - n);
       }
     }
   }
@@ -324,8 +336,8 @@ static int launch_pair_f(const PhW8Pair& p, hipStream_t st) {
 }
 template <int ACT, typename T>
 static int launch_pair_t(const PhW8Pair& p, hipStream_t st) {
-  // 32 tokens a block fill the chip earlier (15088 tokens of 384 -> 512 -> 26: 13.6 against 14.5 us), 64 read the first
-  // weights half as often (30176: 22.4 against 24.0, 120704: 80 against 91)
+  // 32 tokens a block fill the chip earlier (15088 tokens of 384 -> 512 -> 26: 12.5 against 14.2 us), 64 read the first
+  // weights half as often (30176: 20.2 against 21.9, 120704 -> 52: 68 against 80)
   return p.M <= 20000 ? launch_pair_f<2, ACT, T>(p, st) : launch_pair_f<4, ACT, T>(p, st);
 }
 template <int ACT>
