@@ -316,25 +316,30 @@ __global__ __launch_bounds__(64 * W) void w8_few_kernel(const PhW8Params p, cons
   }
 }
 
-// sums of the parts of K -> out; integers, so that their order does not matter
-template <typename O>
+// sums of the parts of K -> out; integers, so that their order does not matter.  J lanes, 64 / J apart, share four channels' parts.
+template <int J, typename O>
 __global__ __launch_bounds__(256) void w8_join_kernel(const PhW8Params p, int parts) {
-  const int q4 = (p.N + 3) / 4;
-  const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (t >= (int64_t)p.M * q4) return;
-  const unsigned m = (unsigned)(t / q4);
-  const int n = (int)(t - (int64_t)m * q4) * 4;
+  const int q4 = (p.N + 3) / 4, lane = threadIdx.x & 63, j = lane / (64 / J);
+  const int64_t pieces = (int64_t)p.M * q4;
+  const int64_t t = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * (64 / J) + lane % (64 / J);
+  const int64_t at_t = min(t, pieces - 1);   // (lanes beyond the end: the last one's again)
+  const unsigned m = (unsigned)(at_t / q4);
+  const int n = (int)(at_t - (int64_t)m * q4) * 4;
   const int64_t pitch = (int64_t)p.M * (p.nnb * 16);
   const int* at = p.parts + (int64_t)m * (p.nnb * 16) + n;
   i32x4 a = i32x4{0, 0, 0, 0};
-  for (int s0 = 0; s0 < parts; s0 += 8) {   // eight at a time on their way
+  for (int s0 = j; s0 < parts; s0 += 8 * J) {   // eight at a time on their way
     i32x4 b[8];
 #pragma unroll
-    for (int s = 0; s < 8; s++) b[s] = s0 + s < parts ? *(const i32x4*)(at + (s0 + s) * pitch) : i32x4{0, 0, 0, 0};
+    for (int s = 0; s < 8; s++) b[s] = s0 + s * J < parts ? *(const i32x4*)(at + (s0 + s * J) * pitch) : i32x4{0, 0, 0, 0};
 #pragma unroll
     for (int s = 0; s < 8; s++) a += b[s];
   }
-  w8_finish4<O>(p, a, m, n, p.qs[m]);
+#pragma unroll
+  for (int d = 64 / J; d < 64; d *= 2)
+#pragma unroll
+    for (int e = 0; e < 4; e++) a[e] += __shfl_xor(a[e], d);
+  if (j == 0 && t < pieces) w8_finish4<O>(p, a, m, n, p.qs[m]);
 }
 
 template <int TM, bool SPLIT, typename O>
@@ -440,7 +445,10 @@ static int launch_product_t(const PhW8Params& p, const PhW8Choice& c, hipStream_
   if (launch_kernel<true, O>(p, c, st)) return -1;
   const int64_t pieces = (int64_t)p.M * ((p.N + 3) / 4);
   if (ph_w8_launchable(pieces, 1)) return -1;
-  hipLaunchKernelGGL((w8_join_kernel<O>), dim3((unsigned)((pieces + 255) / 256)), dim3(256), 0, st, p, c.parts);
+  // few sums of many parts: a lane that adds them all up waits for memory several times over (61 x 32500 -> 187 in 32
+  // parts 11.3 -> 9.5 us)
+  if (c.parts >= 8 && pieces < 65536) hipLaunchKernelGGL((w8_join_kernel<8, O>), dim3((unsigned)((pieces + 31) / 32)), dim3(256), 0, st, p, c.parts);
+  else hipLaunchKernelGGL((w8_join_kernel<1, O>), dim3((unsigned)((pieces + 255) / 256)), dim3(256), 0, st, p, c.parts);
   PH_CHECK(hipGetLastError());
   return 0;
 }
