@@ -318,6 +318,11 @@ int linear(const void* x, int x_type, const PhRowMap& xr, unsigned M, const ph_w
   return ph_launch_w8_product(product_params(w.q, even_rows(pitch), w.s, M, l, out, outr, w.parts, out_type), choice, out_type, st);
 }
 
+int64_t matmul_space(int64_t M, int K, int N, bool even) {
+  const MatmulWay way(M, K, N, even);
+  return RowsSpace(nullptr, way.choice, M, K, N, way.anew, false).used();
+}
+
 // Of two layers: the inner rows in f32, and the larger of the two layers' spaces, one after the other in one place.
 int64_t inner_bytes(int64_t M, int H) { return up(M * up(H, 4) * 4, 256); }
 int64_t pair_space(int64_t M, int K, int H, int N) {
@@ -375,10 +380,10 @@ int64_t ph_w8_workspace(int op, int64_t m, int k, int h, int n) {
   }
   if (m == 0) return 0;
   switch (op) {
-    case PH_W8_MATMUL:
-    case PH_W8_MATMUL_ANY: {
-      const MatmulWay way(m, k, n, op == PH_W8_MATMUL);
-      return RowsSpace(nullptr, way.choice, m, k, n, way.anew, false).used();
+    case PH_W8_MATMUL: return matmul_space(m, k, n, true);
+    case PH_W8_MATMUL_ANY: {   // rows that turn out to be aligned are done the other way
+      const int64_t a = matmul_space(m, k, n, true), b = matmul_space(m, k, n, false);
+      return a > b ? a : b;
     }
     case PH_W8_LINEAR: return linear_space(m, k, n);
     case PH_W8_FEED_FORWARD:

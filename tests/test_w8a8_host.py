@@ -93,6 +93,14 @@ def test_c_refusals():
     assert ff(layer(n=64), layer(k=64, n=0)) == -1
 
 
+def test_workspace_for_any_rows_holds_aligned_ones_too():
+    lib = _ffi.lib()
+    for m in (1, 5, 16, 33, 64, 65, 70, 130, 300, 1000, 5000, 100000):
+        for k in (1, 15, 16, 31, 64, 301, 1001, 4001, 32500, w8a8.MAX_K):
+            for n in (1, 16, 40, 187, 1000, 4096):
+                assert lib.ph_w8_workspace(_ffi.PH_W8_MATMUL_ANY, m, k, 0, n) >= lib.ph_w8_workspace(_ffi.PH_W8_MATMUL, m, k, 0, n) >= 0
+
+
 def test_python_refusals_without_a_gpu():
     x = torch.zeros(2, 4)
     for f in (lambda: w8a8.quantize_rows(x), lambda: w8a8.Layer(x), lambda: w8a8.Layer(x, act="tanh"),
