@@ -111,6 +111,33 @@ def _out_rows(in_shape, in_stride, shape, stride):
 
 
 @lru_cache(maxsize=4096)
+def _apart(shape, stride, size, out_shape, out_stride, out_size, diff):
+    """Whether an output that starts diff bytes behind an input shares no byte with it, as far as that is easily told: it ends
+    before, starts after, or both are parts of one wider buffer (the same strides) that do not meet."""
+    if 0 in shape or 0 in out_shape:
+        return True
+    end = sum((n - 1) * s for n, s in zip(shape, stride)) * size + size
+    out_end = sum((n - 1) * s for n, s in zip(out_shape, out_stride)) * out_size + out_size
+    if diff >= end or diff + out_end <= 0:
+        return True
+    dims = [(s * size, n) for n, s in zip(shape[:-1], stride[:-1]) if n > 1]
+    if dims != [(s * out_size, n) for n, s in zip(out_shape[:-1], out_stride[:-1]) if n > 1] or any(s == 0 for s, _ in dims):
+        return False
+    dims.sort(reverse=True)
+    width, out_width = shape[-1] * size, out_shape[-1] * out_size
+
+    def meet(diff, dims):   # some row of the output, diff + k . strides behind some row of the input, shares a byte with it
+        if not dims:
+            return -out_width < diff < width
+        (s, n), rest = dims[0], dims[1:]
+        reach = sum(t * (m - 1) for t, m in rest) + max(width, out_width)
+        low, high = max(1 - n, -((reach + diff) // s)), min(n - 1, (reach - diff) // s)
+        return high - low > 8 or any(meet(diff + k * s, rest) for k in range(low, high + 1))
+
+    return not meet(diff, dims)
+
+
+@lru_cache(maxsize=4096)
 def _plan(shape, stride, n):
     """_out_rows for a new, contiguous output of n values a row, and that output's shape."""
     out = tuple(shape[:-1]) + (n,)
@@ -239,12 +266,14 @@ def _output(x, n, out, dtype, default):
         raise ValueError(f"out must be {tuple(shape)} f32 / f16 / bf16 on {x.device}, got {tuple(out.shape)} {out.dtype} on {out.device}")
     if out.requires_grad and torch.is_grad_enabled():
         raise ValueError("8-bit layers have no gradient: out must not ask for one")
+    if not _apart(x.shape, x.stride(), x.element_size(), out.shape, out.stride(), out.element_size(), out.data_ptr() - x.data_ptr()):
+        raise ValueError("out shares memory with the rows that are read")
     return (out,) + _out_rows(x.shape, x.stride(), out.shape, out.stride())
 
 
 def matmul(q, scale, layer, out=None, dtype=None):
     """8-bit rows q int8 [.., K] with scale f32 [..] (``quantize_rows``' or any other's) x layer -> [.., N] of ``dtype``
-    (default bf16), or into ``out`` (a tensor or a view; rows must not overlap each other or an input)."""
+    (default bf16), or into ``out`` (a tensor or a view; rows must not overlap each other or an input: rows side by side in a wider buffer are fine)."""
     _check_layer(layer, q)
     if not q.is_cuda or q.dtype != torch.int8 or q.dim() < 1 or q.shape[-1] != layer.k:
         raise ValueError(f"q must be a CUDA int8 tensor [.., {layer.k}], got {q.dtype} {tuple(q.shape)} on {q.device}")
@@ -266,8 +295,8 @@ def matmul(q, scale, layer, out=None, dtype=None):
 
 
 def linear(x, layer, out=None, dtype=None):
-    """Float rows x [.., K] x layer -> [.., N] of ``dtype`` (default x's), or into ``out``: the rows are quantised on the
-    way."""
+    """Float rows x [.., K] x layer -> [.., N] of ``dtype`` (default x's), or into ``out`` (as for ``matmul``; not x
+    itself): the rows are quantised on the way."""
     _check_layer(layer, x)
     _check_x(x, layer.k, "x")
     y, rows, ostride, m = _output(x, layer.n, out, dtype, x.dtype)

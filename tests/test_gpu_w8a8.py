@@ -452,6 +452,22 @@ def test_first_calls_inside_a_capture(w8):
         assert all(torch.equal(p, r) for p, r in zip(o, e))
 
 
+def test_outputs_beside_their_rows_and_over_them(w8):
+    rng = np.random.default_rng(4)
+    w, ws, bias, _ = weights(rng, 40, 40)
+    layer = make(w8, w, ws, bias)
+    buf = rows(rng, 300, 100, "f32").cuda()
+    x, out = buf[:, :40], buf[:, 50:90]
+    want = ref.linear(x.double().cpu().numpy(), w, ws, bias)
+    w8.linear(x, layer, out=out)
+    same(out, want)
+    assert torch.equal(w8.feed_forward(x, layer, layer, out=out), w8.feed_forward(x, layer, layer))
+    for f in (lambda: w8.linear(x, layer, out=x), lambda: w8.linear(x, layer, out=buf[:, 39:79]),
+              lambda: w8.feed_forward(x[1:], layer, layer, out=x[:-1])):
+        with pytest.raises(ValueError, match="shares memory"):
+            f()
+
+
 def test_a_device_that_is_not_there(w8):
     """A call for one is refused, and nothing of it is left for the next call."""
     from posehip import _ffi

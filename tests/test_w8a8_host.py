@@ -135,6 +135,27 @@ def test_output_rows_that_overlap_are_refused():
     w8a8._out_rows(x.shape, x.stride(), torch.Size((4, 6)), torch.empty(4, 9)[:, 2:8].stride())
 
 
+def test_outputs_that_share_memory_with_the_rows_are_refused():
+    b = torch.empty(6, 10, 64)
+    flat = b.view(-1)
+
+    def apart(x, out):
+        return w8a8._apart(x.shape, x.stride(), x.element_size(), out.shape, out.stride(), out.element_size(), out.data_ptr() - x.data_ptr())
+
+    half = flat.view(torch.bfloat16)
+    for x, out, want in (
+            (b, b, False), (b[0], b[0], False), (b[0], b[1], True), (b[1], b[0], True), (b[0, 0], b[0, 0], False),
+            (b[..., :20], b[..., 20:40], True), (b[..., 20:40], b[..., :20], True), (b[..., :20], b[..., 19:40], False),
+            (b[..., 1:20], b[..., 20:], True), (b[..., 30:50], b[..., 49:60], False), (b[:, ::2], b[:, 1::2], True), (b[:, :5], b[:, 5:], True),
+            (b[:, 1:6], b[:, :5], False), (b[..., :20], b.transpose(0, 1)[..., 20:40].contiguous(), True),
+            (b[:4, :4, :20], b[:4, :4].transpose(0, 1)[..., 20:40], False), (b[0, 0], b[0, 1], True), (b[0, 0, :8], b[0, 0, 8:9], True),
+            (b[0, 0, :9], b[0, 0, 8:10], False), (b[0], half.view(6, 10, 128)[0, :, 64:], False), (b[:0], b[:0], True),
+            (b[0, :1].expand(10, 64), b[0], False)):
+        assert apart(x, out) == want, (x.shape, out.shape)
+    wide = half.view(6, 10, 128)
+    assert apart(b[..., :20], wide[..., 40:100]) and not apart(b[..., :20], wide[..., 39:100])
+
+
 def test_plans_mark_the_pairs_that_fit():
     from posehip import caffe_io, graph
     for proto, pairs in ((caffe_io.body25_prototxt(64, 96), 6), (caffe_io.coco_prototxt(64, 96), 12)):
