@@ -21,8 +21,11 @@ __host__ __device__ static inline int64_t ph_row_off(const PhRowMap& r, unsigned
 }
 
 // A launch holds fewer than 2^32 threads: a call of more rows than that is refused.
+static inline bool ph_w8_fits_launch(int64_t blocks, int64_t threads) {
+  return blocks * threads <= 0xff000000ll;   // (counts rounded up to whole blocks still fit)
+}
 static inline int ph_w8_launchable(int64_t blocks, int64_t threads) {
-  if (blocks * threads <= 0xff000000ll) return 0;   // (counts rounded up to whole blocks still fit)
+  if (ph_w8_fits_launch(blocks, threads)) return 0;
   ph_set_error("8-bit layer: %lld blocks of %lld threads are more than a launch holds: take the rows in parts",
                (long long)blocks, (long long)threads);
   return -1;

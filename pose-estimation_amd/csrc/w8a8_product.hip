@@ -232,6 +232,10 @@ __device__ __forceinline__ i32x4 tail_16(i32x4 v, int K) {
   return v;
 }
 
+// Blocks of 64 tokens stand along z, which ends at 65535 of them; with more tokens along y too (folded into x they need a division
+// in every block: 2000000 x 31 -> 16 113 -> 118 us).
+constexpr unsigned FEW_Z = 64 * 65535;
+
 template <int TM, int W, bool SPLIT, typename T, typename O>
 __global__ __launch_bounds__(64 * W) void w8_few_kernel(const PhW8Params p, const FloatRows f) {
   constexpr bool FLOAT = !__is_same(T, int8_t);
@@ -243,7 +247,9 @@ __global__ __launch_bounds__(64 * W) void w8_few_kernel(const PhW8Params p, cons
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int fr = lane & 15, fq = lane >> 4;
   const int nb = blockIdx.x;
-  const unsigned m0 = blockIdx.z * (16 * TM);
+  unsigned t = blockIdx.z;
+  if (TM == 4 && !SPLIT && !FLOAT && p.M > FEW_Z) t = t * gridDim.y + blockIdx.y;
+  const unsigned m0 = t * (16 * TM);
   const int nk = (p.K + 63) >> 6;   // (a fragment of zeros that the weights may end with is left out)
   const int kb0 = SPLIT ? (int)((int64_t)nk * blockIdx.y / gridDim.y) : 0;
   const int kb1 = SPLIT ? (int)((int64_t)nk * (blockIdx.y + 1) / gridDim.y) : nk;
@@ -344,7 +350,9 @@ __global__ __launch_bounds__(256) void w8_join_kernel(const PhW8Params p, int pa
 
 template <int TM, bool SPLIT, typename O>
 static int launch_few(const PhW8Params& p, int parts, hipStream_t st) {
-  hipLaunchKernelGGL((w8_few_kernel<TM, 8, SPLIT, int8_t, O>), dim3(p.nnb, SPLIT ? parts : 1, (p.M - 1) / (16 * TM) + 1), dim3(512), 0, st, p, FloatRows{});
+  const unsigned tokens = (p.M - 1) / (16 * TM) + 1, y = SPLIT ? parts : (p.M - 1) / FEW_Z + 1, z = SPLIT ? tokens : (tokens - 1) / y + 1;
+  if (ph_w8_launchable((int64_t)p.nnb * y * z, 512)) return -1;
+  hipLaunchKernelGGL((w8_few_kernel<TM, 8, SPLIT, int8_t, O>), dim3(p.nnb, y, z), dim3(512), 0, st, p, FloatRows{});
   PH_CHECK(hipGetLastError());
   return 0;
 }
@@ -411,7 +419,8 @@ PhW8Choice ph_w8_choose_loose(int64_t M, int K, int N) {
   const int tm = M > 48 ? 4 : (int)(M + 15) / 16;
   for (int parts = 1; parts <= 8 && parts <= (nkb + 1) / 2; parts *= 2) {
     if (parts > 1 && (float)M * n16 * parts > (float)(1 << 22)) break;
-    const int64_t rounds = ((M + 63) / 64 * (n16 / 16) * parts + 255) / 256;
+    const int64_t blocks = (M + 63) / 64 * (n16 / 16) * parts, rounds = (blocks + 255) / 256;
+    if (!ph_w8_fits_launch(blocks, 512)) break;   // (the tiles' blocks, of 64 channels and 256 threads, are far fewer)
     const float t = 2.5f + (float)rounds * (0.7f + 0.07f * tm * ((nkb + parts - 1) / parts)) + join_us(M, n16, parts);
     if (t < best.us) best = {K_FEW, parts, t};
   }

@@ -1,0 +1,49 @@
+"""CPU: the launches that the entry points of the 8-bit layers make (tests/w8a8_launches.py), held against what a launch may be."""
+import shutil
+
+import pytest
+
+torch = pytest.importorskip("torch")
+import w8a8_launches  # noqa: E402
+
+pytestmark = pytest.mark.skipif(shutil.which("gcc") is None, reason="builds the stand-in for the HIP calls")
+
+
+@pytest.fixture(scope="module")
+def fake(tmp_path_factory):
+    return w8a8_launches.build(tmp_path_factory.mktemp("fake"))
+
+
+def within_limits(launched):
+    for kernel, grid, block, lds in launched:
+        assert grid[1] <= 65535 and grid[2] <= 65535, (kernel, grid)
+        assert all(g * b < 1 << 32 for g, b in zip(grid, block)), (kernel, grid, block)
+        n = 1
+        for v in grid + block:
+            n *= v
+        assert n <= 1 << 32 and min(grid) >= 1, (kernel, grid, block)
+
+
+# up to 64 * 65535 tokens, past them, and past what one launch of the few-token kernel holds
+MANY = [64 * 65535, 64 * 65535 + 1, 5_000_000, 8_000_000, 534_773_760, 534_773_761, 1_000_000_000]
+
+
+@pytest.mark.parametrize("K,N", [(31, 16), (33, 1), (63, 16), (127, 16), (31, 40)])
+def test_rows_of_any_alignment_in_their_millions(fake, K, N):
+    for M, (rc, launched, _) in zip(MANY, w8a8_launches.launches(fake, [dict(op="matmul", M=M, K=K, N=N) for M in MANY])):
+        assert rc == 0 and launched, M
+        within_limits(launched)
+        kernel, grid, _, _ = launched[-1]
+        blocks = grid[1] * grid[2] * 64 if "w8_few" in kernel else grid[0] * 256   # (256 tokens a block at the most)
+        assert blocks >= M, (M, kernel, grid)
+
+
+def test_every_launch_is_within_limits(fake):
+    sizes = [(M, K, N) for M in (1, 17, 64, 65, 3772, 8193, 120704, 1 << 20, 1 << 24) for K in (1, 8, 31, 384, 513, 4096, 131071)
+             for N in (1, 52, 513, 4097, 1 << 20)]
+    calls = [dict(op=op, M=M, K=K, N=N, H=H, gap=gap) for M, K, N in sizes for op, H, gap in
+             (("matmul", 0, -K % 16), ("matmul", 0, 1), ("linear", 0, 0), ("feed_forward", 33, 0), ("quantize", 0, 0))]
+    for c, (rc, launched, _) in zip(calls, w8a8_launches.launches(fake, calls)):
+        assert rc in (0, -1), c
+        assert rc or launched, c
+        within_limits(launched)
