@@ -2,6 +2,7 @@
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
+#include <mutex>
 
 typedef __bf16 bf16;
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -96,12 +97,17 @@ void ph_set_error(const char* fmt, ...);
 
 // hipFuncAttributeMaxDynamicSharedMemorySize is a per-device property of a kernel: remember, per kernel and
 // device, the largest size already granted (`cache` = a zero-initialised static int[PH_MAX_DEVICES] per kernel).
+// Setting it and remembering it are one step for all threads: else a smaller call's size could be set last and the
+// larger one's be remembered.
 #define PH_MAX_DEVICES 64
+inline std::mutex ph_lds_lock;
 static inline int ph_ensure_lds(const void* fn, int bytes, int* cache) {
   int dev = 0;
   if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= PH_MAX_DEVICES) dev = 0;
+  if (__atomic_load_n(&cache[dev], __ATOMIC_ACQUIRE) >= bytes) return 0;
+  std::lock_guard<std::mutex> lock(ph_lds_lock);
   if (cache[dev] >= bytes) return 0;
   PH_CHECK(hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
-  cache[dev] = bytes;
+  __atomic_store_n(&cache[dev], bytes, __ATOMIC_RELEASE);
   return 0;
 }

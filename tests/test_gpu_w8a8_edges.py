@@ -39,3 +39,30 @@ def test_rows_of_any_alignment_in_their_millions(w8, M, K, N):
     c = [torch.from_numpy(a).cuda() for a in (w, ws, bias)]
     for a in range(0, M, 1 << 20):
         assert torch.equal(y[a:a + (1 << 20)], on_gpu(q[a:a + (1 << 20)], s[a:a + (1 << 20)], *c)), a
+
+
+def test_threads_of_different_widths(w8):
+    """First calls of a kernel at once, with different amounts of LDS."""
+    import threading
+    rng = np.random.default_rng(3)
+    a = weights(rng, 512, 64)
+    l1 = make(w8, a[0], a[1], a[2], "none")
+    second = [weights(rng, n, 512) for n in (64, 48, 33, 17)]
+    layers = [make(w8, *b[:3]) for b in second]
+    x = rows(rng, 20500, 64, "f32")
+    d = x.cuda()
+    torch.cuda.synchronize()
+    got = [None] * 4
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(3):
+                y = w8.feed_forward(d, l1, layers[i])
+            torch.cuda.current_stream().synchronize()
+            got[i] = y.cpu()
+
+    ts = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    [t.start() for t in ts]
+    [t.join() for t in ts]
+    for b, g in zip(second, got):
+        same(g, ref.feed_forward(x.double().numpy(), (a[0], a[1], a[2], "none"), b[:3] + ("none", None)))

@@ -15,13 +15,14 @@ def fake(tmp_path_factory):
 
 
 def within_limits(launched):
-    for kernel, grid, block, lds in launched:
+    for kernel, grid, block, lds, most in launched:
         assert grid[1] <= 65535 and grid[2] <= 65535, (kernel, grid)
         assert all(g * b < 1 << 32 for g, b in zip(grid, block)), (kernel, grid, block)
         n = 1
         for v in grid + block:
             n *= v
         assert n <= 1 << 32 and min(grid) >= 1, (kernel, grid, block)
+        assert lds <= most, (kernel, lds, most)
 
 
 # up to 64 * 65535 tokens, past them, and past what one launch of the few-token kernel holds
@@ -30,10 +31,10 @@ MANY = [64 * 65535, 64 * 65535 + 1, 5_000_000, 8_000_000, 534_773_760, 534_773_7
 
 @pytest.mark.parametrize("K,N", [(31, 16), (33, 1), (63, 16), (127, 16), (31, 40)])
 def test_rows_of_any_alignment_in_their_millions(fake, K, N):
-    for M, (rc, launched, _) in zip(MANY, w8a8_launches.launches(fake, [dict(op="matmul", M=M, K=K, N=N) for M in MANY])):
+    for M, (rc, launched) in zip(MANY, w8a8_launches.launches(fake, [dict(op="matmul", M=M, K=K, N=N) for M in MANY])):
         assert rc == 0 and launched, M
         within_limits(launched)
-        kernel, grid, _, _ = launched[-1]
+        kernel, grid = launched[-1][:2]
         blocks = grid[1] * grid[2] * 64 if "w8_few" in kernel else grid[0] * 256   # (256 tokens a block at the most)
         assert blocks >= M, (M, kernel, grid)
 
@@ -43,7 +44,21 @@ def test_every_launch_is_within_limits(fake):
              for N in (1, 52, 513, 4097, 1 << 20)]
     calls = [dict(op=op, M=M, K=K, N=N, H=H, gap=gap) for M, K, N in sizes for op, H, gap in
              (("matmul", 0, -K % 16), ("matmul", 0, 1), ("linear", 0, 0), ("feed_forward", 33, 0), ("quantize", 0, 0))]
-    for c, (rc, launched, _) in zip(calls, w8a8_launches.launches(fake, calls)):
+    for c, (rc, launched) in zip(calls, w8a8_launches.launches(fake, calls)):
         assert rc in (0, -1), c
         assert rc or launched, c
         within_limits(launched)
+
+
+@pytest.mark.parametrize("large,small", [(dict(op="feed_forward", M=30000, K=64, H=512, N=64), dict(op="feed_forward", M=30000, K=64, H=512, N=48)),
+                                         (dict(op="linear", M=64, K=512, N=64), dict(op="linear", M=60, K=512, N=64))])
+@pytest.mark.parametrize("t", [0, 1, 2])
+def test_two_first_calls_of_a_kernel_at_once(fake, large, small, t):
+    """Calls of one kernel that need different amounts of LDS, the smaller one's on another thread while the larger one's is
+    being granted: what is granted never gets less again."""
+    large, small = dict(large, t=t), dict(small, t=t)
+    for rc, launched in w8a8_launches.launches(fake, [dict(large, beside=small), large, small, large]):
+        assert rc == 0 and launched
+        within_limits(launched)
+    (_, a), (_, b) = w8a8_launches.launches(fake, [large, small])
+    assert a[0][0] == b[0][0] and a[0][3] > b[0][3]
