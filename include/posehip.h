@@ -304,8 +304,8 @@ typedef struct {
   int64_t stride[3];
 } ph_rows;
 /* A layer: n output channels, k inputs (k <= 131071: the int32 sum cannot overflow; n <= 2^20).  scale / bias / slope
- * hold n values rounded up to a multiple of 16, each array 16-byte aligned; bias may be NULL, slope may be NULL unless act
- * is PH_ACT_PRELU. */
+ * hold n values rounded up to a multiple of 16 (those from n on may be anything), each array 16-byte aligned; bias may be
+ * NULL, slope may be NULL unless act is PH_ACT_PRELU. */
 typedef struct {
   const int8_t* packed; /* ph_w8_pack's output */
   const float* scale;

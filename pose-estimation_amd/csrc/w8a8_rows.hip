@@ -195,7 +195,7 @@ __global__ __launch_bounds__(512, 4) void w8_pair_kernel(const PhW8Pair p) {
   // (from cache, so here before the rows, which loads that return in order would hold up otherwise)
   for (int f = wave; f < p.nnb2 * p.nkb2; f += 8)
     __builtin_amdgcn_global_load_lds((glb_void*)(p.w2 + f * 1024 + lane * 16), (lds_void*)(w2 + f * 1024), 16, 0, 0);
-  const bool is = tid < p.nnb1 * 16;   // (channels that do not exist: zeros)
+  const bool is = tid < p.nnb1 * 16;
   float out_par = 0.f;
   if (tid < 3 * 64 && (tid & 63) < p.nnb2 * 16) {
     const float* const from = tid < 64 ? p.ws2 : tid < 128 ? p.bias2 : p.slope2;
@@ -205,7 +205,8 @@ __global__ __launch_bounds__(512, 4) void w8_pair_kernel(const PhW8Pair p) {
 #pragma unroll
   for (int j = 0; j < 4; j++) wa[j] = *(const i32x4*)wp[j];
   rows_to_lds<TF, T>(p.x, p.xr, p.M, p.K, m0, q, s1, tid, [&] {});
-  par[tid] = par0_, par[PAIR_MAX + tid] = par1_, par[2 * PAIR_MAX + tid] = par2_;
+  const bool exists = tid < p.H;   // channels that do not: zeros, whatever stands in their places, as all enter the rows' maxima
+  par[tid] = exists ? par0_ : 0.f, par[PAIR_MAX + tid] = exists ? par1_ : 0.f, par[2 * PAIR_MAX + tid] = exists ? par2_ : 0.f;
   if (tid < 3 * 64) par2[tid] = out_par;
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the second layer's weights are in LDS (as the rows, requested after them)
   __syncthreads();

@@ -66,3 +66,20 @@ def test_threads_of_different_widths(w8):
     [t.join() for t in ts]
     for b, g in zip(second, got):
         same(g, ref.feed_forward(x.double().numpy(), (a[0], a[1], a[2], "none"), b[:3] + ("none", None)))
+
+
+@pytest.mark.parametrize("junk", [float("nan"), float("inf"), -1e38, 1e30])
+@pytest.mark.parametrize("M,K,H,N", [(77, 100, 1, 21), (77, 100, 33, 21), (77, 100, 500, 21), (20100, 40, 33, 5), (77, 100, 600, 70), (9000, 64, 33, 300)])
+def test_padding_of_parameters_may_be_anything(w8, M, K, H, N, junk):
+    """Scale, bias and slope of the channels from n to the next multiple of 16."""
+    rng = np.random.default_rng(H)
+    a, b = weights(rng, H, K), weights(rng, N, H)
+    x = rows(rng, M, K, "f32").cuda()
+    l1, l2 = make(w8, a[0], a[1], a[2], "prelu", a[3]), make(w8, b[0], b[1], b[2], "prelu", b[3])
+    want = w8.feed_forward(x, l1, l2), w8.linear(x, l1), w8.linear(x[:5], l1), w8.matmul(*w8.quantize_rows(x), l1)
+    l1._par[:, H:] = junk
+    l2._par[:, N:] = junk
+    got = w8.feed_forward(x, l1, l2), w8.linear(x, l1), w8.linear(x[:5], l1), w8.matmul(*w8.quantize_rows(x), l1)
+    for y, z in zip(got, want):
+        assert torch.isfinite(z).all() and torch.equal(y, z)
+    same(got[0], ref.feed_forward(x.double().cpu().numpy(), (a[0], a[1], a[2], "prelu", a[3]), (b[0], b[1], b[2], "prelu", b[3])))
