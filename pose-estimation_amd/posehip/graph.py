@@ -203,7 +203,7 @@ def _build_nodes(net, height, width):
 
 def _mark_w8a8(plan):
     """Pairs of 1x1 layers that the 8-bit kernel takes (PH_OP_CONV_W8A8): the first one's output read by the second only,
-    at most 512 -> 512 -> 64 channels."""
+    which reads nothing else, at most 512 -> 512 -> 64 channels."""
     readers = {}
     for o in plan.ops:
         readers[o["in_buf"]] = readers.get(o["in_buf"], 0) + 1
@@ -213,6 +213,8 @@ def _mark_w8a8(plan):
         if len(a["dst"]) != 1 or a["f32_coff"] >= 0 or a["dst"][0] != (b["in_buf"], b["in_coff"]):
             continue
         if readers[b["in_buf"]] != 1 or a["cin_read"] > 512 or a["cout"] > 512 or b["cin_read"] > 512 or b["cout"] > 64:
+            continue
+        if (b["cin_map"][a["cout"]:] >= 0).any():   # (a concatenation that the first one is a part of)
             continue
         a["w8a8"] = b["w8a8"] = True
 

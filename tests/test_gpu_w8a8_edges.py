@@ -83,3 +83,20 @@ def test_padding_of_parameters_may_be_anything(w8, M, K, H, N, junk):
     for y, z in zip(got, want):
         assert torch.isfinite(z).all() and torch.equal(y, z)
     same(got[0], ref.feed_forward(x.double().cpu().numpy(), (a[0], a[1], a[2], "prelu", a[3]), (b[0], b[1], b[2], "prelu", b[3])))
+
+
+def test_networks_whose_pairs_do_not_fit(engine):
+    """They run as they do without 8 bits."""
+    from posehip import _ffi, graph, synth
+    from test_gpu_net import _tiny_net
+    from test_w8a8_plans import NETS
+    for spec, pairs in NETS.values():
+        net = _tiny_net(16, 24, spec)
+        w = graph.random_weights(net, seed=1, out_gain=1.0)
+        outs = []
+        for w8a8 in (False, True):
+            engine.build(graph.build_plan(net, w, w8a8=w8a8), 2)
+            engine.preprocess(synth.synth_frames(2, 2, 16, 24), _ffi.PH_PRE_CV2)
+            engine.forward(2)
+            outs.append(engine.net_out(2))
+        assert np.array_equal(*outs) == (pairs == 0) and np.isfinite(outs[0]).all()
