@@ -138,6 +138,23 @@ def _apart(shape, stride, size, out_shape, out_stride, out_size, diff):
 
 
 @lru_cache(maxsize=4096)
+def _clear_of(size, out_shape, out_stride, out_size, diff):
+    """Whether an output of rows that do not overlap, diff bytes behind one piece of `size` bytes, shares no byte with it."""
+    if 0 in out_shape or not size:
+        return True
+    dims = sorted(((s * out_size, n) for n, s in zip(out_shape[:-1], out_stride[:-1]) if n > 1), reverse=True)
+
+    def meet(low, high, dims):   # bytes low .. high - 1, from the output's first on, hold one of a row's
+        if not dims:
+            return low < out_shape[-1] * out_size and high > 0
+        (s, n), rest = dims[0], dims[1:]
+        a, b = max(low // s, 0), min((high - 1) // s, n - 1)
+        return b - a > 1 or any(meet(low - k * s, high - k * s, rest) for k in range(a, b + 1))   # (between two: a whole step)
+
+    return not meet(-diff, size - diff, dims)
+
+
+@lru_cache(maxsize=4096)
 def _plan(shape, stride, n):
     """_out_rows for a new, contiguous output of n values a row, and that output's shape."""
     out = tuple(shape[:-1]) + (n,)
@@ -284,6 +301,8 @@ def matmul(q, scale, layer, out=None, dtype=None):
     if not scale.is_contiguous():
         scale = scale.contiguous()
     y, rows, ostride, m = _output(q, layer.n, out, dtype, torch.bfloat16)
+    if out is not None and not _clear_of(scale.numel() * 4, out.shape, out.stride(), out.element_size(), out.data_ptr() - scale.data_ptr()):
+        raise ValueError("out shares memory with the scales that are read")
     if m:
         even = not (q.data_ptr() % 16 or rows.stride[0] % 16 or rows.stride[1] % 16 or rows.stride[2] % 16)
         need = _workspace(_ffi.PH_W8_MATMUL if even else _ffi.PH_W8_MATMUL_ANY, m, layer.k, 0, layer.n)

@@ -100,3 +100,26 @@ def test_networks_whose_pairs_do_not_fit(engine):
             engine.forward(2)
             outs.append(engine.net_out(2))
         assert np.array_equal(*outs) == (pairs == 0) and np.isfinite(outs[0]).all()
+
+
+def test_outputs_over_scales(w8):
+    rng = np.random.default_rng(5)
+    w, ws, bias, _ = weights(rng, 20, 64)
+    layer = make(w8, w, ws, bias)
+    x = rows(rng, 30, 64, "f32").cuda()
+    q, s = w8.quantize_rows(x)
+    want = w8.matmul(q, s, layer, dtype=torch.float32)
+    wide = torch.zeros(30 * 40 + 60, device="cuda")
+    out = wide[30:30 + 1200].view(30, 40)[:, :20]
+    for lo, ok in ((0, True), (1, False), (40, False), (1200, False), (1210, True), (1230, True)):
+        sc = wide[lo:lo + 30]
+        sc.copy_(s)
+        if ok:
+            w8.matmul(q, sc, layer, out=out)
+            assert torch.equal(out, want) and torch.equal(sc, s)
+        else:
+            with pytest.raises(ValueError, match="scales"):
+                w8.matmul(q, sc, layer, out=out)
+    over = torch.zeros(30, 22, device="cuda")   # scales that are not side by side are copied first: their place may be written
+    over[:, 3] = s
+    assert torch.equal(w8.matmul(q, over[:, 3], layer, out=over[:, 1:21]), want)
