@@ -17,7 +17,7 @@ The sum is an exact 32-bit integer (K <= 131071), each later operation is rounde
 so ``linear(x, l)`` is ``matmul(*quantize_rows(x), l)`` and ``feed_forward(x, a, b)`` is
 ``linear(linear(x, a, dtype=torch.float32), b)``, both bit for bit, whatever the sizes.  A row with a NaN or an infinity
 gives NaN outputs and touches no other row.  There are no gradients: inputs and outputs that ask
-for one are refused (a Layer takes a parameter's values as they are).
+for one, or carry a tangent (forward mode), are refused (a Layer takes a parameter's values as they are).
 
 Tensors are CUDA tensors of f32 / f16 / bf16 with the values of a row consecutive (last stride 1) and any other strides;
 leading dimensions that do not merge into three are refused.  Work is put on torch's current stream of the tensors'
@@ -29,6 +29,7 @@ import ctypes as C
 from functools import lru_cache
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _ffi
 
@@ -173,12 +174,17 @@ def _workspace(op, m, k, h, n):
     return b
 
 
+def _wants_gradient(t):
+    """In either direction: a tensor that requires one, or that carries a tangent."""
+    return t.requires_grad and torch.is_grad_enabled() or forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None
+
+
 def _check_x(x, k, what):
     if not x.is_cuda or x.dtype not in _TYPES:
         raise ValueError(f"{what} must be a CUDA tensor of f32, f16 or bf16, got {x.dtype} on {x.device}")
     if x.dim() < 1 or (k is not None and x.shape[-1] != k):
         raise ValueError(f"{what} must be [.., {k}], got {tuple(x.shape)}")
-    if x.requires_grad and torch.is_grad_enabled():
+    if _wants_gradient(x):
         raise ValueError("8-bit layers have no gradient: call them under torch.no_grad() or detach their inputs")
 
 
@@ -281,7 +287,7 @@ def _output(x, n, out, dtype, default):
     shape = x.shape[:-1] + (n,)
     if out.shape != shape or out.device != x.device or out.dtype not in _TYPES or (dtype is not None and dtype != out.dtype):
         raise ValueError(f"out must be {tuple(shape)} f32 / f16 / bf16 on {x.device}, got {tuple(out.shape)} {out.dtype} on {out.device}")
-    if out.requires_grad and torch.is_grad_enabled():
+    if _wants_gradient(out):
         raise ValueError("8-bit layers have no gradient: out must not ask for one")
     if not _apart(x.shape, x.stride(), x.element_size(), out.shape, out.stride(), out.element_size(), out.data_ptr() - x.data_ptr()):
         raise ValueError("out shares memory with the rows that are read")
@@ -296,7 +302,7 @@ def matmul(q, scale, layer, out=None, dtype=None):
         raise ValueError(f"q must be a CUDA int8 tensor [.., {layer.k}], got {q.dtype} {tuple(q.shape)} on {q.device}")
     if scale.shape != q.shape[:-1] or scale.dtype != torch.float32 or scale.device != q.device:
         raise ValueError(f"scale must be f32 {tuple(q.shape[:-1])} on {q.device}, got {scale.dtype} {tuple(scale.shape)} on {scale.device}")
-    if scale.requires_grad and torch.is_grad_enabled():
+    if _wants_gradient(scale):
         raise ValueError("8-bit layers have no gradient: call them under torch.no_grad() or detach their inputs")
     if not scale.is_contiguous():
         scale = scale.contiguous()

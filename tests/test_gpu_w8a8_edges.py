@@ -123,3 +123,27 @@ def test_outputs_over_scales(w8):
     over = torch.zeros(30, 22, device="cuda")   # scales that are not side by side are copied first: their place may be written
     over[:, 3] = s
     assert torch.equal(w8.matmul(q, over[:, 3], layer, out=over[:, 1:21]), want)
+
+
+def test_tangents_are_refused(w8):
+    """Forward mode, also without gradients in the other direction; a detached tensor has none."""
+    from torch.autograd import forward_ad as fw
+    rng = np.random.default_rng(0)
+    w, ws, bias, _ = weights(rng, 32, 32)
+    layer = make(w8, w, ws, bias)
+    x = torch.randn(4, 32, device="cuda")
+    want = w8.linear(x, layer)
+    q, s = w8.quantize_rows(x)
+    with fw.dual_level():
+        d, ds, out = (fw.make_dual(t, torch.ones_like(t)) for t in (x.clone(), s.clone(), torch.empty(4, 32, device="cuda")))
+        for mode in (torch.enable_grad, torch.no_grad):
+            with mode():
+                for f in (lambda: w8.linear(d, layer), lambda: w8.quantize_rows(d), lambda: w8.feed_forward(d, layer, layer),
+                          lambda: w8.matmul(q, ds, layer), lambda: w8.linear(x, layer, out=out)):
+                    with pytest.raises(ValueError, match="no gradient"):
+                        f()
+        assert torch.equal(w8.linear(x, layer), want) and torch.equal(w8.linear(d.detach(), layer), want)
+        W = torch.randn(20, 32, device="cuda")
+        dual = w8.Layer(fw.make_dual(W, torch.ones_like(W)), bias=fw.make_dual(W[:, 0].contiguous(), torch.ones(20, device="cuda")))
+        assert torch.equal(w8.linear(x, dual), w8.linear(x, w8.Layer(W, bias=W[:, 0])))
+    assert torch.equal(w8.linear(x, layer), want)
