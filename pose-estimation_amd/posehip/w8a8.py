@@ -17,7 +17,8 @@ The sum is an exact 32-bit integer (K <= 131071), each later operation is rounde
 so ``linear(x, l)`` is ``matmul(*quantize_rows(x), l)`` and ``feed_forward(x, a, b)`` is
 ``linear(linear(x, a, dtype=torch.float32), b)``, both bit for bit, whatever the sizes.  A row with a NaN or an infinity
 gives NaN outputs and touches no other row.  There are no gradients: inputs and outputs that ask
-for one, or carry a tangent (forward mode), are refused (a Layer takes a parameter's values as they are).
+for one, or carry a tangent (forward mode), are refused (a Layer takes a parameter's values as they are); so are the tensors that
+torch.func's transforms hand out.
 
 Tensors are CUDA tensors of f32 / f16 / bf16 with the values of a row consecutive (last stride 1) and any other strides;
 leading dimensions that do not merge into three are refused.  Work is put on torch's current stream of the tensors'
@@ -36,10 +37,6 @@ from . import _ffi
 _TYPES = {torch.float32: _ffi.PH_F32, torch.float16: _ffi.PH_F16, torch.bfloat16: _ffi.PH_BF16}
 _ACTS = {"none": _ffi.PH_ACT_NONE, "relu": _ffi.PH_ACT_RELU, "prelu": _ffi.PH_ACT_PRELU}
 MAX_K = 131071
-
-
-def _stream(device):
-    return _raw_stream(device.index)
 
 
 # torch.cuda.current_stream().cuda_stream without the Stream object around it (0.1 against 1.9 us a call)
@@ -176,7 +173,19 @@ def _workspace(op, m, k, h, n):
 
 def _wants_gradient(t):
     """In either direction: a tensor that requires one, or that carries a tangent."""
-    return t.requires_grad and torch.is_grad_enabled() or forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None
+    if t.requires_grad and torch.is_grad_enabled():
+        return True
+    return forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None
+
+
+_transforms = torch._C._functorch.maybe_current_level
+
+
+def _check_memory(*tensors):
+    """The transforms of torch.func hand out tensors without memory of their own."""
+    for t in tensors + (torch.empty(0),):
+        if t is not None and torch._C._functorch.is_functorch_wrapped_tensor(t):
+            raise ValueError("8-bit layers read and write memory: the transforms of torch.func do not go through them")
 
 
 def _check_x(x, k, what):
@@ -197,6 +206,8 @@ def quantize_rows(x):
     """x [.., K] float -> (q int8 [.., K], scale f32 [..]); x ~ q * scale[.., None].  q's rows start at multiples of 16
     bytes (a view of a wider buffer where K is no multiple of 16)."""
     _check_x(x, None, "x")
+    if _transforms() is not None:
+        _check_memory(x)
     shape, device = x.shape, x.device
     k = shape[-1]
     if k < 1:
@@ -224,6 +235,8 @@ class Layer:
             raise ValueError(f"act must be one of {sorted(_ACTS)}, got {act!r}")
         if not weight.is_cuda:
             raise ValueError("weight must be a CUDA tensor")
+        if _transforms() is not None:
+            _check_memory(weight, scale, bias, slope)
         weight = weight.detach()
         if weight.dim() == 4 and tuple(weight.shape[2:]) == (1, 1):
             weight = weight[:, :, 0, 0]
@@ -260,7 +273,7 @@ class Layer:
         self.packed = torch.empty(nbytes, dtype=torch.int8, device=dev)
         self.n, self.k, self.act, self.device = n, k, act, dev
         self._par = par
-        _ffi.check(lib.ph_w8_pack(dev.index, _stream(dev), q.data_ptr(), q.stride(0) if n > 1 else k, n, k,
+        _ffi.check(lib.ph_w8_pack(dev.index, _raw_stream(dev.index), q.data_ptr(), q.stride(0) if n > 1 else k, n, k,
                                   self.packed.data_ptr()), "ph_w8_pack")
         row = par.stride(0) * 4
         self.desc = _ffi.PhW8Layer(self.packed.data_ptr(), par.data_ptr(), par.data_ptr() + row if bias is not None else None,
@@ -304,6 +317,8 @@ def matmul(q, scale, layer, out=None, dtype=None):
         raise ValueError(f"scale must be f32 {tuple(q.shape[:-1])} on {q.device}, got {scale.dtype} {tuple(scale.shape)} on {scale.device}")
     if _wants_gradient(scale):
         raise ValueError("8-bit layers have no gradient: call them under torch.no_grad() or detach their inputs")
+    if _transforms() is not None:
+        _check_memory(q, scale, out)
     if not scale.is_contiguous():
         scale = scale.contiguous()
     y, rows, ostride, m = _output(q, layer.n, out, dtype, torch.bfloat16)
@@ -313,7 +328,8 @@ def matmul(q, scale, layer, out=None, dtype=None):
         even = not (q.data_ptr() % 16 or rows.stride[0] % 16 or rows.stride[1] % 16 or rows.stride[2] % 16)
         need = _workspace(_ffi.PH_W8_MATMUL if even else _ffi.PH_W8_MATMUL_ANY, m, layer.k, 0, layer.n)
         ws = torch.empty(need, dtype=torch.int8, device=q.device) if need else None
-        _ffi.check(_ffi.lib().ph_w8_matmul(q.device.index, _stream(q.device), q.data_ptr(), rows, scale.data_ptr(), layer.desc,
+        device = q.device.index
+        _ffi.check(_ffi.lib().ph_w8_matmul(device, _raw_stream(device), q.data_ptr(), rows, scale.data_ptr(), layer.desc,
                                            y.data_ptr(), _TYPES[y.dtype], ostride, ws.data_ptr() if need else None, need),
                    "ph_w8_matmul")
     return y
@@ -324,11 +340,14 @@ def linear(x, layer, out=None, dtype=None):
     itself): the rows are quantised on the way."""
     _check_layer(layer, x)
     _check_x(x, layer.k, "x")
+    if _transforms() is not None:
+        _check_memory(x, out)
     y, rows, ostride, m = _output(x, layer.n, out, dtype, x.dtype)
     if m:
         need = _workspace(_ffi.PH_W8_LINEAR, m, layer.k, 0, layer.n)
         ws = torch.empty(need, dtype=torch.int8, device=x.device) if need else None
-        _ffi.check(_ffi.lib().ph_w8_linear(x.device.index, _stream(x.device), x.data_ptr(), _TYPES[x.dtype], rows, layer.desc,
+        device = x.device.index
+        _ffi.check(_ffi.lib().ph_w8_linear(device, _raw_stream(device), x.data_ptr(), _TYPES[x.dtype], rows, layer.desc,
                                            y.data_ptr(), _TYPES[y.dtype], ostride, ws.data_ptr() if need else None, need),
                    "ph_w8_linear")
     return y
@@ -340,13 +359,16 @@ def feed_forward(x, layer1, layer2, out=None, dtype=None):
     _check_layer(layer1, x)
     _check_layer(layer2, x)
     _check_x(x, layer1.k, "x")
+    if _transforms() is not None:
+        _check_memory(x, out)
     if layer1.n != layer2.k:
         raise ValueError(f"the first layer has {layer1.n} outputs, the second {layer2.k} inputs")
     y, rows, ostride, m = _output(x, layer2.n, out, dtype, x.dtype)
     if m:
         need = _workspace(_ffi.PH_W8_FEED_FORWARD, m, layer1.k, layer1.n, layer2.n)
         ws = torch.empty(need, dtype=torch.int8, device=x.device) if need else None
-        _ffi.check(_ffi.lib().ph_w8_feed_forward(x.device.index, _stream(x.device), x.data_ptr(), _TYPES[x.dtype], rows,
+        device = x.device.index
+        _ffi.check(_ffi.lib().ph_w8_feed_forward(device, _raw_stream(device), x.data_ptr(), _TYPES[x.dtype], rows,
                                                  layer1.desc, layer2.desc, y.data_ptr(), _TYPES[y.dtype], ostride,
                                                  ws.data_ptr() if need else None, need), "ph_w8_feed_forward")
     return y

@@ -147,3 +147,26 @@ def test_tangents_are_refused(w8):
         dual = w8.Layer(fw.make_dual(W, torch.ones_like(W)), bias=fw.make_dual(W[:, 0].contiguous(), torch.ones(20, device="cuda")))
         assert torch.equal(w8.linear(x, dual), w8.linear(x, w8.Layer(W, bias=W[:, 0])))
     assert torch.equal(w8.linear(x, layer), want)
+
+
+def test_transforms_are_refused(w8):
+    rng = np.random.default_rng(0)
+    w, ws, bias, _ = weights(rng, 32, 32)
+    layer = make(w8, w, ws, bias)
+    x, W = torch.randn(4, 32, device="cuda"), torch.from_numpy(w).cuda()
+    q, s = w8.quantize_rows(x)
+    S, out = torch.from_numpy(ws).cuda(), torch.empty(4, 32, device="cuda")
+    calls = [(x, lambda t: w8.linear(t, layer)), (x, lambda t: w8.quantize_rows(t)[1]), (x, lambda t: w8.feed_forward(t, layer, layer)),
+             (s, lambda t: w8.matmul(q, t.expand(4), layer)), (x, lambda t: w8.linear(x, layer, out=t.expand(4, 32))),
+             (S, lambda t: w8.Layer(W, scale=S, bias=t).packed), (x, lambda t: w8.Layer(t.expand(4, 32)).packed)]
+    for t, f in calls:
+        for transform in (torch.func.vmap(f), torch.func.functionalize(f), torch.func.grad(lambda v: f(v).sum()),
+                          lambda v: torch.func.jvp(f, (v,), (torch.ones_like(v),))):
+            with pytest.raises(ValueError):
+                transform(t)
+    with pytest.raises(ValueError):
+        torch.func.vmap(lambda t: w8.matmul(t, s[0], layer))(q)
+    with pytest.raises(ValueError):
+        torch.func.functionalize(lambda t: w8.linear(x, layer) + t)(out)
+    torch.func.vmap(lambda t: t + w8.linear(x, layer))(out)   # (x is no tensor of the transform's)
+    assert torch.equal(w8.linear(x, layer), w8.matmul(q, s, layer, dtype=torch.float32))
