@@ -289,6 +289,10 @@ def _check_layer(layer, x):
         raise ValueError(f"the layer is on {layer.device}, the rows on {x.device}")
 
 
+# autograd's count of writes: a tensor that was saved for a gradient and then written by a kernel is noticed
+_written = torch.autograd.graph.increment_version
+
+
 def _output(x, n, out, dtype, default):
     """(out, ph_rows of x, strides of out, number of rows)"""
     if out is None:
@@ -332,6 +336,8 @@ def matmul(q, scale, layer, out=None, dtype=None):
         _ffi.check(_ffi.lib().ph_w8_matmul(device, _raw_stream(device), q.data_ptr(), rows, scale.data_ptr(), layer.desc,
                                            y.data_ptr(), _TYPES[y.dtype], ostride, ws.data_ptr() if need else None, need),
                    "ph_w8_matmul")
+        if out is not None:
+            _written(out)
     return y
 
 
@@ -350,6 +356,8 @@ def linear(x, layer, out=None, dtype=None):
         _ffi.check(_ffi.lib().ph_w8_linear(device, _raw_stream(device), x.data_ptr(), _TYPES[x.dtype], rows, layer.desc,
                                            y.data_ptr(), _TYPES[y.dtype], ostride, ws.data_ptr() if need else None, need),
                    "ph_w8_linear")
+        if out is not None:
+            _written(out)
     return y
 
 
@@ -371,4 +379,6 @@ def feed_forward(x, layer1, layer2, out=None, dtype=None):
         _ffi.check(_ffi.lib().ph_w8_feed_forward(device, _raw_stream(device), x.data_ptr(), _TYPES[x.dtype], rows,
                                                  layer1.desc, layer2.desc, y.data_ptr(), _TYPES[y.dtype], ostride,
                                                  ws.data_ptr() if need else None, need), "ph_w8_feed_forward")
+        if out is not None:
+            _written(out)
     return y

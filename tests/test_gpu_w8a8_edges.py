@@ -170,3 +170,29 @@ def test_transforms_are_refused(w8):
         torch.func.functionalize(lambda t: w8.linear(x, layer) + t)(out)
     torch.func.vmap(lambda t: t + w8.linear(x, layer))(out)   # (x is no tensor of the transform's)
     assert torch.equal(w8.linear(x, layer), w8.matmul(q, s, layer, dtype=torch.float32))
+
+
+def test_writes_into_tensors_that_a_gradient_needs_are_noticed(w8):
+    rng = np.random.default_rng(0)
+    w, ws, bias, _ = weights(rng, 32, 32)
+    layer = make(w8, w, ws, bias)
+    x = torch.randn(4, 32, device="cuda")
+    q, s = w8.quantize_rows(x)
+    for f in (lambda out: w8.linear(x, layer, out=out), lambda out: w8.feed_forward(x, layer, layer, out=out),
+              lambda out: w8.matmul(q, s, layer, out=out)):
+        buf = torch.rand(4, 40, device="cuda")
+        p = torch.ones(4, 40, device="cuda", requires_grad=True)
+        y = (buf * p).sum()
+        f(buf[:, :32])
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+        y = (buf * p).sum()   # after the write: its values
+        y.backward()
+        assert torch.equal(p.grad, buf)
+    with torch.inference_mode():
+        out = torch.empty(4, 32, device="cuda")
+        assert torch.equal(w8.linear(x, layer, out=out), w8.linear(x, layer))
+    w8.linear(x, layer, out=out)   # (an inference tensor has no count)
+    empty = torch.empty(0, 32, device="cuda")
+    w8.linear(x[:0], layer, out=empty)
+    assert empty._version == 0
