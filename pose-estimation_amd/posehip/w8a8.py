@@ -105,6 +105,7 @@ def _out_rows(in_shape, in_stride, shape, stride):
     r, os = _ffi.PhRows(), (C.c_int64 * 3)()
     for i, (n, s, o) in enumerate(dims):
         r.n[i], r.stride[i], os[i] = n, s, o
+    r.by_16 = all(s % 16 == 0 for _, s, _ in dims)   # (of 8-bit rows)
     return r, os, m
 
 
@@ -191,7 +192,8 @@ def _check_memory(*tensors):
 def _check_x(x, k, what):
     if not x.is_cuda or x.dtype not in _TYPES:
         raise ValueError(f"{what} must be a CUDA tensor of f32, f16 or bf16, got {x.dtype} on {x.device}")
-    if x.dim() < 1 or (k is not None and x.shape[-1] != k):
+    shape = x.shape
+    if not shape or (k is not None and shape[-1] != k):
         raise ValueError(f"{what} must be [.., {k}], got {tuple(x.shape)}")
     if _wants_gradient(x):
         raise ValueError("8-bit layers have no gradient: call them under torch.no_grad() or detach their inputs")
@@ -206,6 +208,8 @@ def quantize_rows(x):
     """x [.., K] float -> (q int8 [.., K], scale f32 [..]); x ~ q * scale[.., None].  q's rows start at multiples of 16
     bytes (a view of a wider buffer where K is no multiple of 16)."""
     _check_x(x, None, "x")
+    if x.is_neg():
+        x = x.resolve_neg()
     if _transforms() is not None:
         _check_memory(x)
     shape, device = x.shape, x.device
@@ -237,7 +241,7 @@ class Layer:
             raise ValueError("weight must be a CUDA tensor")
         if _transforms() is not None:
             _check_memory(weight, scale, bias, slope)
-        weight = weight.detach()
+        weight = weight.detach().resolve_neg()
         if weight.dim() == 4 and tuple(weight.shape[2:]) == (1, 1):
             weight = weight[:, :, 0, 0]
         if weight.dim() != 2 or weight.shape[0] < 1 or weight.shape[1] < 1:
@@ -304,6 +308,8 @@ def _output(x, n, out, dtype, default):
     shape = x.shape[:-1] + (n,)
     if out.shape != shape or out.device != x.device or out.dtype not in _TYPES or (dtype is not None and dtype != out.dtype):
         raise ValueError(f"out must be {tuple(shape)} f32 / f16 / bf16 on {x.device}, got {tuple(out.shape)} {out.dtype} on {out.device}")
+    if out.is_neg():
+        raise ValueError("out must hold its values as they are, not negated (torch.Tensor.is_neg)")
     if _wants_gradient(out):
         raise ValueError("8-bit layers have no gradient: out must not ask for one")
     if not _apart(x.shape, x.stride(), x.element_size(), out.shape, out.stride(), out.element_size(), out.data_ptr() - x.data_ptr()):
@@ -323,14 +329,15 @@ def matmul(q, scale, layer, out=None, dtype=None):
         raise ValueError("8-bit layers have no gradient: call them under torch.no_grad() or detach their inputs")
     if _transforms() is not None:
         _check_memory(q, scale, out)
-    if not scale.is_contiguous():
-        scale = scale.contiguous()
+    if q.is_neg():
+        q = q.resolve_neg()
+    if scale.is_neg() or not scale.is_contiguous():
+        scale = scale.resolve_neg().contiguous()
     y, rows, ostride, m = _output(q, layer.n, out, dtype, torch.bfloat16)
     if out is not None and not _clear_of(scale.numel() * 4, out.shape, out.stride(), out.element_size(), out.data_ptr() - scale.data_ptr()):
         raise ValueError("out shares memory with the scales that are read")
     if m:
-        even = not (q.data_ptr() % 16 or rows.stride[0] % 16 or rows.stride[1] % 16 or rows.stride[2] % 16)
-        need = _workspace(_ffi.PH_W8_MATMUL if even else _ffi.PH_W8_MATMUL_ANY, m, layer.k, 0, layer.n)
+        need = _workspace(_ffi.PH_W8_MATMUL if rows.by_16 and not q.data_ptr() % 16 else _ffi.PH_W8_MATMUL_ANY, m, layer.k, 0, layer.n)
         ws = torch.empty(need, dtype=torch.int8, device=q.device) if need else None
         device = q.device.index
         _ffi.check(_ffi.lib().ph_w8_matmul(device, _raw_stream(device), q.data_ptr(), rows, scale.data_ptr(), layer.desc,
@@ -346,6 +353,8 @@ def linear(x, layer, out=None, dtype=None):
     itself): the rows are quantised on the way."""
     _check_layer(layer, x)
     _check_x(x, layer.k, "x")
+    if x.is_neg():
+        x = x.resolve_neg()
     if _transforms() is not None:
         _check_memory(x, out)
     y, rows, ostride, m = _output(x, layer.n, out, dtype, x.dtype)
@@ -367,6 +376,8 @@ def feed_forward(x, layer1, layer2, out=None, dtype=None):
     _check_layer(layer1, x)
     _check_layer(layer2, x)
     _check_x(x, layer1.k, "x")
+    if x.is_neg():
+        x = x.resolve_neg()
     if _transforms() is not None:
         _check_memory(x, out)
     if layer1.n != layer2.k:

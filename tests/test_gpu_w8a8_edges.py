@@ -196,3 +196,26 @@ def test_writes_into_tensors_that_a_gradient_needs_are_noticed(w8):
     empty = torch.empty(0, 32, device="cuda")
     w8.linear(x[:0], layer, out=empty)
     assert empty._version == 0
+
+
+def test_negated_views(w8):
+    """Tensors whose memory holds the values' negatives: the imaginary part of a conjugate, and what torch makes like it."""
+    rng = np.random.default_rng(0)
+    w, ws, bias, _ = weights(rng, 20, 1)
+    one, layer = make(w8, w, ws, bias), make(w8, *weights(rng, 64, 64)[:3])
+    x = torch.randn(4, 1, dtype=torch.complex64, device="cuda").conj().imag
+    y = torch._neg_view(torch.randn(4, 64, device="cuda"))
+    q, s = w8.quantize_rows(y.clone())
+    nq, ns = torch._neg_view(q), torch._neg_view(s)
+    assert all(t.is_neg() for t in (x, y, nq, ns))
+    for f, t, l in ((w8.linear, x, one), (w8.linear, y, layer)):
+        assert torch.equal(f(t, l), f(t.clone(), l))
+    assert torch.equal(w8.feed_forward(y, layer, layer), w8.feed_forward(y.clone(), layer, layer))
+    assert torch.equal(w8.quantize_rows(y)[0], q)
+    assert torch.equal(w8.matmul(nq, s, layer), w8.matmul(-q, s, layer)) and torch.equal(w8.matmul(q, ns, layer), w8.matmul(q, -s, layer))
+    W = torch._neg_view(torch.randn(32, 64, device="cuda"))
+    b = torch._neg_view(torch.randn(32, device="cuda"))
+    assert torch.equal(w8.linear(y, w8.Layer(W, bias=b)), w8.linear(y, w8.Layer(W.clone(), bias=b.clone())))
+    assert torch.equal(w8.Layer(nq, scale=s).packed, w8.Layer(-q, scale=s).packed)
+    with pytest.raises(ValueError, match="negated"):
+        w8.linear(y, layer, out=torch._neg_view(torch.empty(4, 64, device="cuda")))
