@@ -12,7 +12,8 @@ runs batch 1) and the ``posehip_*`` keys of the params dict:
                            missing ``model_folder`` raises FileNotFoundError
   posehip_device         : GPU index (default 0)
   posehip_batch          : max frames per call (default 1)
-  posehip_w8a8           : the 1x1 layers that close a stage in 8-bit integers (default False)
+  posehip_w8a8           : the 1x1 layers that close a stage in 8-bit integers (default False; a truth value or one of
+                           ``utils.str2bool``'s words)
 """
 import argparse
 import math
@@ -24,6 +25,7 @@ import numpy as np
 from . import _ffi, caffe_io, draw, graph
 from .engine import Engine
 from .tables import TORSO_IDS, V2_MODELS  # noqa: F401  (TORSO_IDS re-exported)
+from .utils import as_bool
 
 _MODEL_FILES = {
     "BODY_25": ("pose/body_25/pose_deploy.prototxt", "pose/body_25/pose_iter_584000.caffemodel"),
@@ -106,6 +108,7 @@ class Wrapper:
         if name not in V2_MODELS:
             raise ValueError(f"model_pose {name!r} not supported (have {sorted(V2_MODELS)})")
         self._model = V2_MODELS[name]
+        as_bool(p.get("posehip_w8a8", False))   # (refused here, not by the first frame)
         folder = p.get("model_folder", "/usr/local/src/openpose/models/")
         proto, weights = (os.path.join(folder, f) for f in _MODEL_FILES[name])
         if os.path.exists(proto) and os.path.exists(weights):
@@ -138,7 +141,7 @@ class Wrapper:
         key = (net_w, net_h)
         if self._built is None or self._built[:2] != key or self._built[2] < batch:
             plan = graph.build_plan(self._net, self._weights, height=net_h, width=net_w,
-                                    w8a8=bool(self.params.get("posehip_w8a8", False)))
+                                    w8a8=as_bool(self.params.get("posehip_w8a8", False)))
             cap = max(batch, int(self.params.get("posehip_batch", 1)))
             self._engine.build(plan, cap)
             self._built = (net_w, net_h, cap)

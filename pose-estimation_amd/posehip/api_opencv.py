@@ -16,6 +16,7 @@ import numpy as np
 from . import _ffi, caffe_io, draw, graph
 from .engine import Engine
 from .tables import COLORS, MAPIDX, get_body_parts_and_pose_pairs  # noqa: F401
+from .utils import as_bool
 
 
 class _Net:
@@ -57,7 +58,7 @@ class PyOpenPoseOpenCV:
         """Loads the Caffe model (``readNetFromCaffe``, skeleton.py:39-53).  ``cuda``
         is accepted for compatibility; the network always runs on the MI355X.  w8a8: the 1x1 layers that close a
         stage in 8-bit integers."""
-        self._w8a8 = bool(w8a8)
+        self._w8a8 = as_bool(w8a8)
         if os.path.exists(proto_file):
             with open(proto_file) as f:
                 self._parsed = caffe_io.parse_prototxt(f.read())

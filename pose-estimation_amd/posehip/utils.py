@@ -66,6 +66,16 @@ def str2bool(v: str) -> bool:
     raise argparse.ArgumentTypeError('Boolean value expected.')
 
 
+def as_bool(v) -> bool:
+    """A parameter that is on or off: a truth value, a number, None, or one of :func:`str2bool`'s words."""
+    if isinstance(v, str):
+        try:
+            return str2bool(v)
+        except argparse.ArgumentTypeError:
+            raise ValueError(f"on or off expected, got {v!r}") from None
+    return bool(v)
+
+
 def cosine_distance(a: np.ndarray, b: np.ndarray, data_is_normalized: bool = False) -> np.ndarray:
     """Pairwise ``1 - cos`` between the rows of a [N,M] and b [L,M] -> [N,L] (``utils.py:75-97``)."""
     if not data_is_normalized:

@@ -219,3 +219,18 @@ def test_negated_views(w8):
     assert torch.equal(w8.Layer(nq, scale=s).packed, w8.Layer(-q, scale=s).packed)
     with pytest.raises(ValueError, match="negated"):
         w8.linear(y, layer, out=torch._neg_view(torch.empty(4, 64, device="cuda")))
+
+
+def test_estimator_parameter_in_words_and_in_a_namespace():
+    import argparse
+    from posehip import api_native, synth
+    frame = synth.synth_frames(3, 1, 120, 160)[0]
+    args = argparse.Namespace(op_model_folder="/nonexistent/", op_model_pose="BODY_25", op_net_resolution="160x128", op_heatmaps_add_parts=False,
+                              op_heatmaps_add_bkg=False, op_heatmaps_add_PAFs=False, op_heatmaps_scale=1, op_display=0, op_skel_thres=0.0,
+                              op_max_true_body=8, op_patch_offset=2, posehip_random_weights=0)
+    for value, on in (("0", False), ("yes", True), (False, False), (True, True), (None, False)):
+        args.posehip_w8a8 = value
+        pe = api_native.OpenPosePoseExtractor(args)
+        pe.predict(frame, None)
+        assert any(k.startswith("w8_pair") for k in pe.pyop.opWrapper._engine.op_kernels()) == on
+        pe.pyop.opWrapper.close()
