@@ -62,3 +62,30 @@ def test_two_first_calls_of_a_kernel_at_once(fake, large, small, t):
         within_limits(launched)
     (_, a), (_, b) = w8a8_launches.launches(fake, [large, small])
     assert a[0][0] == b[0][0] and a[0][3] > b[0][3]
+
+
+def test_the_products_tested_on_the_gpu_take_every_kernel(fake):
+    import itertools
+    from test_gpu_w8a8_kernels import PRODUCTS
+    calls = [dict(op="matmul", M=M, K=K, N=N, gap=-K % 16) for _, _, M, K, N in PRODUCTS]
+    taken = set()
+    for (kernel, split, M, K, N), (rc, launched) in zip(PRODUCTS, w8a8_launches.launches(fake, calls)):
+        assert rc == 0 and kernel in launched[0][0] and len(launched) == 1 + split, (M, K, N, launched)
+        within_limits(launched)
+        taken.add((kernel, split))
+    # no size of a grid over the range takes another one
+    sizes = [2 ** i for i in range(0, 18, 2)], [16, 96, 384, 1536, 6144, 24576, 98304], [1, 16, 64, 130, 520, 2080, 8320, 33280]
+    calls = [dict(op="matmul", M=M, K=K, N=N) for M, K, N in itertools.product(*sizes)]
+    for c, (rc, launched) in zip(calls, w8a8_launches.launches(fake, calls)):
+        assert rc == 0 and any(k in launched[0][0] and split == (len(launched) == 2) for k, split in taken), (c, launched)
+
+
+def test_the_layers_tested_on_the_gpu_take_every_kernel(fake):
+    from test_gpu_w8a8_kernels import FEED_FORWARD, LINEAR, QUANTIZE
+    want = [(f"quantize_rows_kernelI{c}Li{lanes}E", dict(op="quantize", M=M, K=K, t=t)) for lanes, M, K in QUANTIZE
+            for t, c in ((0, "f"), (1, "DF16_"), (2, "DF16b"))]
+    want += [(k, dict(op="linear", M=M, K=K, N=N)) for k, M, K, N in LINEAR]
+    want += [(k, dict(op="feed_forward", M=M, K=K, H=H, N=N)) for k, M, K, H, N in FEED_FORWARD]
+    for (kernel, c), (rc, launched) in zip(want, w8a8_launches.launches(fake, [c for _, c in want])):
+        assert rc == 0 and kernel in launched[0][0], (c, launched)
+        within_limits(launched)
