@@ -169,9 +169,9 @@ int ph_launch_w8_rows(const PhW8Params& p, const FloatRows& f, int x_type, int o
 // (weights straight from cache, each fragment read by one wave and used for TF products); inner values and their maxima;
 // inner rows in 8 bits into the same LDS; second product, its weights in LDS for good.  Two blocks share a CU, so that one's
 // rounding (12 vector operations per inner value) runs under the other's products.
-// 120704 x 384 -> 512 -> 52 bf16: 68 us (its bytes 22, its products 22).  Of a block's 15.6 us: rows 1.6, their rounding 3.0,
-// waiting for each other 1.3, first product 2.9, inner values 2.2, their rounding 2.3, second product 1.3, output 1.0: the vector
-// units bound it, busy for 40 us of the 68 (fma, add, mul take 2 cycles a wave; conversions, maxima, compares, shifts 4).
+// 120704 x 384 -> 512 -> 52 bf16: 59 .. 64 us (its bytes 22, its products 22 at 2.4 POP/s).  Per SIMD 24.8 k vector instructions
+// (43 us at 4 cycles each, less as fma, add, mul take 2) and 1650 matrix instructions (11 us); a wave waits for memory, LDS or
+// its block 43 % of its time and for another wave's instruction 24 %.
 constexpr int AHEAD = 512;   // blocks that run at a time: two on each of 256 CUs
 
 template <int TF, int ACT, typename T>
@@ -214,7 +214,7 @@ __global__ __launch_bounds__(512, 4) void w8_pair_kernel(const PhW8Pair p) {
   i32x4 acc[4][TF];
   rows_product<TF>(xq, wp, wa, p.nkb1, acc);
   // A line of each 128 bytes of the rows that the block after the next on this CU will read: its loads find them in L2
-  // (2.4 -> 1.6 us a block).
+  // (120704 x 384 -> 512 -> 52 74 -> 72.5 us).
   T ahead = T(0.f);
   if (TF == 4) {
     const int64_t m = (int64_t)m0 + AHEAD * BT + (tid >> 3);
@@ -337,8 +337,8 @@ static int launch_pair_f(const PhW8Pair& p, hipStream_t st) {
 }
 template <int ACT, typename T>
 static int launch_pair_t(const PhW8Pair& p, hipStream_t st) {
-  // 32 tokens a block fill the chip earlier (15088 tokens of 384 -> 512 -> 26: 12.5 against 14.2 us), 64 read the first
-  // weights half as often (30176: 20.2 against 21.9, 120704 -> 52: 68 against 80)
+  // 32 tokens a block fill the chip earlier (3772 tokens of 384 -> 512 -> 26: 7.7 against 11.3 us, 15088: 11.1 against 12.2), 64 read
+  // the first weights half as often (30176: 16.5 against 18.6, 120704 -> 52: 59 against 69); 20000: 15.6 and 16.0
   return p.M <= 20000 ? launch_pair_f<2, ACT, T>(p, st) : launch_pair_f<4, ACT, T>(p, st);
 }
 template <int ACT>
